@@ -279,6 +279,59 @@ long long lw_host_pairs(const uint8_t* codes, int N, int K, int fmt, const uint8
                         uint32_t* table, long long table_cap, uint32_t* group_base, long long group_base_cap,
                         uint32_t* words, long long words_cap);
 
+/* ---- paged key-value cache (additions) --------------------------------------------------------------------
+ *
+ * Keys and values of several sequences in two pools of pages, [n_pages][n_kv_heads][page_size][head_dim] in fp16 or bf16
+ * with any strides (of elements, multiples of 8; head_dim contiguous), which the caller owns.  The reference holds one
+ * sequence in one contiguous fp16 cache (kernels/llmrt.cu:1305-1332, :1336-1498); these entry points are what several
+ * sequences in one pass need, and have no counterpart there.
+ *
+ * Sequence b has lens[b] positions, those of the call's rows included, in the pages table[b * table_stride + 0 ..]; entries
+ * behind its length are not read.  Its rows are starts[b] .. starts[b + 1] - 1 (starts: n_seqs + 1 ascending values) and hold
+ * its LAST positions, in order; rows before starts[0] and from starts[n_seqs] on belong to no sequence.  lens, table and starts
+ * are read on the device, when the kernel runs: a captured call can be replayed with other lengths, pages and rows.
+ * A page index outside the pool, a length beyond the table's columns or a position beyond the rotation tables is not
+ * followed: nothing is written there, what is read there is undefined, and bit 1 of the device error word (lw_kernel_error) is
+ * set.  All pointers but the handle are device pointers; calls launch on `stream` and do not synchronise. */
+enum { LW_TYPE_F16 = 0, LW_TYPE_BF16 = 1, LW_TYPE_F32 = 2 };
+
+/* A handle on two pools (nothing is allocated on the device).  n_kv_heads >= 1, page_size a multiple of 8 up to 65536, head_dim a
+ * multiple of 8 up to 128, pools on 16-byte boundaries.  Belongs to the current device.  NULL and lw_last_status on failure.
+ * lw_cache_destroy frees the handle only. */
+void* lw_cache_create(void* k_pages, void* v_pages, int type, int n_pages, int n_kv_heads, int page_size, int head_dim,
+                      long long page_stride, long long head_stride, long long token_stride);
+void lw_cache_destroy(void* cache);
+
+/* Rows of a fused product, [n_rows][n_heads + 2 n_kv_heads][head_dim] of qkv_type with row_stride elements between rows, at any
+ * address the type allows: queries rotated to their positions into q [row][head][head_dim], keys rotated and values as they
+ * are into the pages, each rounded once to the cache's type.  Rotation of the pairs (i, i + rope_half), i < rope_half, by
+ * cos_table / sin_table[position][rope_half]; dimensions from 2 rope_half on are copied.  rope_half: a multiple of 4.
+ * starts may be null: one row per sequence, row b the last position of sequence b (rows from n_seqs on belong to none).
+ * Rows of no sequence, and rows before position 0 (more rows than lens[b]), are left alone, in q too. */
+int lw_cache_append(void* cache, const void* qkv, int qkv_type, long long row_stride, int n_rows, int n_heads, const float* cos_table,
+                    const float* sin_table, int rope_rows, int rope_half, const int* starts, const int* lens, const int* table,
+                    int n_seqs, int table_cols, long long table_stride, void* q, long long q_token_stride, long long q_head_stride,
+                    void* stream);
+
+/* Bytes of workspace that attention over n_rows rows of n_heads heads needs (0: none, a null workspace will do); prompt: of
+ * lw_cache_attend_prompt.  The caller owns it, on a 16-byte boundary; its contents do not matter.  Calls that overlap on the
+ * GPU - captured ones too - need one each. */
+long long lw_cache_workspace(void* cache, int n_rows, int n_heads, int prompt);
+
+/* Attention of one new token per sequence: out[b][h] = sum_j softmax_j(scale q[b][h] . k_j) v_j over the positions
+ * max(0, lens[b] - window) <= j < lens[b] (window 0: from 0).  Query head h reads kv head h / (n_heads / n_kv_heads).  q and out in
+ * the cache's type, rows and heads on 16-byte boundaries.  A sequence of length 0 gives zeros. */
+int lw_cache_attend(void* cache, const void* q, long long q_token_stride, long long q_head_stride, int n_seqs, int n_heads, const int* lens,
+                    const int* table, int table_cols, long long table_stride, float scale, int window, void* out,
+                    long long out_token_stride, long long out_head_stride, void* workspace, long long workspace_bytes, void* stream);
+
+/* The same for the rows of packed prompts, or of pieces of prompts whose beginnings are in the pages already: the row at position p
+ * sees max(0, p - window + 1) .. p.  A row before position 0 sees nothing and gives zeros; rows of no sequence are left alone. */
+int lw_cache_attend_prompt(void* cache, const void* q, long long q_token_stride, long long q_head_stride, int n_rows, int n_heads,
+                           const int* starts, const int* lens, const int* table, int n_seqs, int table_cols, long long table_stride,
+                           float scale, int window, void* out, long long out_token_stride, long long out_head_stride, void* workspace,
+                           long long workspace_bytes, void* stream);
+
 /* ---- diagnostics ------------------------------------------------------------------------------------------ */
 
 /* Message of the last failure on the calling thread. */
@@ -287,7 +340,8 @@ const char* lw_last_error(void);
 /* Status code of the last rt_open / lw_matrix_create on the calling thread (they can only return NULL). */
 int lw_last_status(void);
 
-/* Reads and clears the device error word (bit 0: a bounded wait on a bulk copy gave up).  After a non-zero answer the
+/* Reads and clears the device error word (bit 0: a bounded wait on a bulk copy gave up; bit 1: a kernel of the paged cache met
+ * a page, length or position that it did not follow).  After a non-zero answer the
  * results of products that were in flight are undefined; the next product of every matrix first zeroes the matrix's
  * tile-row counters again, so later products are correct. */
 int lw_kernel_error(void);

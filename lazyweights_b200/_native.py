@@ -69,6 +69,18 @@ _SIGNATURES = {
     "lw_ngram_destroy": (None, [C.c_void_p]),
     "lw_ngram_push": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int]),
     "lw_ngram_draft": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int]),
+    "lw_cache_create": (C.c_void_p, [C.c_void_p, C.c_void_p] + [C.c_int] * 5 + [C.c_longlong] * 3),
+    "lw_cache_destroy": (None, [C.c_void_p]),
+    "lw_cache_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
+                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_longlong, C.c_void_p, C.c_longlong,
+                                  C.c_longlong, C.c_void_p]),
+    "lw_cache_workspace": (C.c_longlong, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
+    "lw_cache_attend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
+                                  C.c_longlong, C.c_float, C.c_int, C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p, C.c_longlong,
+                                  C.c_void_p]),
+    "lw_cache_attend_prompt": (C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
+                                         C.c_void_p, C.c_int, C.c_int, C.c_longlong, C.c_float, C.c_int, C.c_void_p, C.c_longlong,
+                                         C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p]),
     "lw_debug_set": (C.c_int, [C.c_char_p, C.c_longlong]),
     "lw_debug_wait_probe": (C.c_int, [C.c_longlong]),
     "lw_last_error": (C.c_char_p, []),

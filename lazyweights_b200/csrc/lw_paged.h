@@ -1,0 +1,53 @@
+// The paged key-value cache: geometry handle, launchers of the kernels that fill and read it (lw_paged.cu: appending with
+// the position rotation, C ABI; lw_attend.cuh / .cu: attention).
+#pragma once
+#include <cuda.h>
+
+#include "lw_gemv1.h"
+
+namespace lw {
+
+enum ElemType { kF16 = 0, kBF16 = 1, kF32 = 2 };
+
+// The error word's bit for indexes that the kernels refused to follow (lw_kernel_error): a page outside the pool, a length
+// beyond the page table's columns, a position beyond the rotation tables.
+constexpr unsigned int kErrWordIndex = 2u;
+
+// The two pools as the kernels see them; strides in elements, the head dimension is contiguous.
+struct PagePool {
+  void *k, *v;
+  long long page_stride, head_stride, token_stride;
+  int n_pages, Hk, page_size, Dh;
+};
+
+struct PagedCache {
+  PagePool pool;
+  ElemType type;
+  int device = -1;   // -1: made without a CUDA device; nothing can be launched on it
+};
+
+// Which positions belong to which rows: sequence b owns rows starts[b] .. starts[b + 1] - 1 (row b alone if starts is null),
+// the last of its lens[b] positions; its pages are table[b * table_stride + 0 .. table_cols - 1].
+struct Sequences {
+  const int *starts, *lens, *table;
+  long long table_stride;
+  int n, table_cols;
+};
+
+// Arguments of attention: q and out rows [head][Dh], strides in elements.
+struct AttendArgs {
+  PagePool pool;
+  Sequences seq;
+  const void* q;
+  void* out;
+  long long q_token, q_head, out_token, out_head;
+  int H, rows;        // query heads, rows of q
+  int window;         // 0: none
+  float scale;
+  void* workspace;
+  unsigned int* err;
+};
+
+int launch_attend(ElemType type, const AttendArgs& a, cudaStream_t st);
+
+}  // namespace lw

@@ -1,0 +1,167 @@
+"""Keys and values of several sequences in pools of pages, and the operators that fill and read them.
+
+`append` rotates the rows of a fused q/k/v product and writes their keys and values to the pages; `attend` is attention of
+one new token per sequence, `attend_prompt` causal attention of packed prompts (or pieces of prompts).  All three take the
+same description of the sequences, CUDA int32 tensors that are read when the kernel runs (a captured call can be replayed
+with other contents):
+
+  table   [n, columns]  the pages of every sequence; entries behind its length are not read
+  lens    [n]           length of every sequence, the positions of the call's rows included
+  starts  [n + 1]       rows starts[b] .. starts[b + 1] - 1 are the last positions of sequence b; rows outside belong to none
+
+torch is only used for device memory and streams.  A page outside the pool, a length beyond the table or a position beyond
+the rotation tables is not followed and sets bit 1 of lw_kernel_error().
+"""
+from . import _native as nat
+from .runtime import _stream, _torch
+
+_CODES = None
+
+
+def _codes(torch):
+    global _CODES
+    if _CODES is None:
+        _CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+    return _CODES
+
+
+class PagedCache:
+    """Pools k_pages and v_pages [pages, kv_heads, page_size, head_dim], CUDA fp16 or bf16, of the same strides (any multiples of
+    eight, head_dim contiguous: a pool with the heads inside the positions is passed transposed).  The tensors are kept alive."""
+
+    def __init__(self, k_pages, v_pages):
+        torch = _torch()
+        self._h = None
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype is not v_pages.dtype or \
+                k_pages.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("PagedCache wants two fp16 or bf16 pools [pages, kv_heads, page_size, head_dim] of one shape and type")
+        if not k_pages.is_cuda or k_pages.device != v_pages.device:
+            raise ValueError("the pools must be on one CUDA device")
+        n, heads, size, dim = k_pages.shape
+        sp, sh, st, sd = k_pages.stride()
+        if sd != 1 or any(a != b and c > 1 for a, b, c in zip(k_pages.stride(), v_pages.stride(), k_pages.shape)):
+            raise ValueError("the pools must have the same strides and a contiguous head_dim")
+        self.k_pages, self.v_pages = k_pages, v_pages
+        self.n_pages, self.kv_heads, self.page_size, self.head_dim = n, heads, size, dim
+        self.dtype, self.device, self._index = k_pages.dtype, k_pages.device, k_pages.get_device()
+        with torch.cuda.device(self._index):
+            ptr = nat.lib().lw_cache_create(k_pages.data_ptr(), v_pages.data_ptr(), _codes(torch)[self.dtype], n, heads, size, dim, sp, sh, st)
+        if not ptr:
+            raise nat.LwError(nat.lib().lw_last_status() or -1, nat.last_error())
+        self._h = ptr
+
+    @classmethod
+    def empty(cls, n_pages, kv_heads, page_size, head_dim, dtype=None, device="cuda"):
+        """A cache with pools of its own (fp16 unless `dtype` says otherwise)."""
+        torch = _torch()
+        shape = (n_pages, kv_heads, page_size, head_dim)
+        pools = [torch.empty(shape, dtype=dtype or torch.float16, device=device) for _ in range(2)]
+        return cls(*pools)
+
+    def close(self):
+        if self._h:
+            nat.lib().lw_cache_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    # ---- checks
+    def _sequences(self, torch, table, lens):
+        i32 = torch.int32
+        if table.dtype is not i32 or lens.dtype is not i32 or table.dim() != 2 or lens.dim() != 1 or table.shape[0] != lens.shape[0] or \
+                table.get_device() != self._index or lens.get_device() != self._index:
+            raise ValueError("table [n, columns] and lens [n] must be int32 on the cache's device")
+        n, cols = table.shape
+        if cols > 1 and table.stride(1) != 1 or n > 1 and lens.stride(0) != 1:
+            raise ValueError("the rows of table, and lens, must be contiguous")
+        return n, cols, table.stride(0) if n > 1 else max(cols, 1)
+
+    def _starts(self, torch, starts, n):
+        if starts.dtype is not torch.int32 or starts.dim() != 1 or starts.shape[0] != n + 1 or starts.get_device() != self._index or \
+                starts.stride(0) != 1:
+            raise ValueError("starts [%d] must be contiguous int32 on the cache's device" % (n + 1))
+
+    def _rows(self, t, what, rows=None, heads=None):
+        """Strides of a [rows, heads, head_dim] tensor of queries or results."""
+        if t.dim() != 3 or t.dtype is not self.dtype or t.get_device() != self._index or t.shape[2] != self.head_dim or t.stride(2) != 1 or \
+                (rows is not None and (t.shape[0] != rows or t.shape[1] != heads)):
+            raise ValueError("%s must be [rows, heads, %d] of the cache's type and device, head_dim contiguous" % (what, self.head_dim))
+        r, h = t.shape[0], t.shape[1]
+        sh = t.stride(1) if h > 1 else self.head_dim
+        return (t.stride(0) if r > 1 else h * sh), sh
+
+    # ---- operators
+    def append(self, qkv, n_heads, cos, sin, table, lens, starts=None, q=None):
+        """Rows [n, (n_heads + 2 kv_heads) * head_dim] (fp16, bf16 or fp32) of a fused product: rotated queries [n, n_heads,
+        head_dim] in the cache's type are returned (`q`: a tensor to fill), rotated keys and values go to the pages.  cos, sin: fp32
+        tables [positions, r], pairs (i, i + r) are rotated, dimensions from 2 r on copied.  Without starts, row b is the last position
+        of sequence b.  Rows of no sequence are left as they are, in q too."""
+        torch = _torch()
+        n, cols, tstride = self._sequences(torch, table, lens)
+        if starts is not None:
+            self._starts(torch, starts, n)
+        code = _codes(torch).get(qkv.dtype)
+        if qkv.dim() != 2 or code is None or qkv.get_device() != self._index or qkv.shape[1] != (n_heads + 2 * self.kv_heads) * self.head_dim or \
+                qkv.stride(1) != 1:
+            raise ValueError("qkv must be [rows, %d] fp16, bf16 or fp32 on the cache's device" % ((n_heads + 2 * self.kv_heads) * self.head_dim))
+        f32 = torch.float32
+        if cos.dtype is not f32 or sin.dtype is not f32 or cos.dim() != 2 or cos.shape != sin.shape or not cos.is_contiguous() or \
+                not sin.is_contiguous() or cos.get_device() != self._index or sin.get_device() != self._index:
+            raise ValueError("cos and sin must be contiguous fp32 tables [positions, pairs] on the cache's device")
+        rows = qkv.shape[0]
+        if q is None:
+            q = torch.empty((rows, n_heads, self.head_dim), dtype=self.dtype, device=self.device)
+        qt, qh = self._rows(q, "q", rows, n_heads)
+        rc = nat.lib().lw_cache_append(self._h, qkv.data_ptr(), code, qkv.stride(0) if rows > 1 else qkv.shape[1], rows, n_heads,
+                                       cos.data_ptr(), sin.data_ptr(), cos.shape[0], cos.shape[1],
+                                       None if starts is None else starts.data_ptr(), lens.data_ptr(), table.data_ptr(), n, cols, tstride,
+                                       q.data_ptr(), qt, qh, _stream(torch, self._index))
+        if rc < 0:
+            nat.check(rc)
+        return q
+
+    def _workspace(self, torch, rows, heads, prompt):
+        need = nat.check(nat.lib().lw_cache_workspace(self._h, rows, heads, prompt))
+        return torch.empty(need, dtype=torch.uint8, device=self.device) if need else None, need
+
+    def attend(self, q, table, lens, scale=None, window=0, out=None):
+        """Attention of one new token per sequence: q [n, heads, head_dim] -> the same shape (`out`: a tensor to fill).  scale: of
+        the scores, head_dim ** -0.5 unless given; window: positions seen, the token's own included (0: all).  A sequence of length 0
+        gives zeros."""
+        torch = _torch()
+        n, cols, tstride = self._sequences(torch, table, lens)
+        qt, qh = self._rows(q, "q", n, q.shape[1])
+        if out is None:
+            out = torch.empty((n, q.shape[1], self.head_dim), dtype=self.dtype, device=self.device)
+        ot, oh = self._rows(out, "out", n, q.shape[1])
+        space, size = self._workspace(torch, n, q.shape[1], 0)
+        rc = nat.lib().lw_cache_attend(self._h, q.data_ptr(), qt, qh, n, q.shape[1], lens.data_ptr(), table.data_ptr(), cols, tstride,
+                                       self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(), ot, oh,
+                                       space.data_ptr() if size else None, size, _stream(torch, self._index))
+        if rc < 0:
+            nat.check(rc)
+        return out
+
+    def attend_prompt(self, q, table, lens, starts, scale=None, window=0, out=None):
+        """Causal attention of packed rows q [rows, heads, head_dim] -> the same shape: rows starts[b] .. starts[b + 1] - 1 are the last
+        positions of sequence b, each sees the positions up to its own (with a window, the last `window` of them).  Rows before
+        position 0 give zeros, rows of no sequence are left as they are."""
+        torch = _torch()
+        n, cols, tstride = self._sequences(torch, table, lens)
+        self._starts(torch, starts, n)
+        qt, qh = self._rows(q, "q")
+        rows, heads = q.shape[0], q.shape[1]
+        if out is None:
+            out = torch.empty((rows, heads, self.head_dim), dtype=self.dtype, device=self.device)
+        ot, oh = self._rows(out, "out", rows, heads)
+        space, size = self._workspace(torch, rows, heads, 1)
+        rc = nat.lib().lw_cache_attend_prompt(self._h, q.data_ptr(), qt, qh, rows, heads, starts.data_ptr(), lens.data_ptr(), table.data_ptr(),
+                                              n, cols, tstride, self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
+                                              ot, oh, space.data_ptr() if size else None, size, _stream(torch, self._index))
+        if rc < 0:
+            nat.check(rc)
+        return out
