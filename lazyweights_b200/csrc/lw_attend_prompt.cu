@@ -1,0 +1,645 @@
+// Causal attention of packed prompts over the paged cache, on the tensor cores.
+//
+//   O[row, :] = sum_j softmax_j(scale Q[row] . K[j]) V[j]        rows = (token, head of the group) of one kv head
+//
+// One pass over the positions with a running reference m of the scores (in powers of two): p = 2^(c s - m), l = sum p,
+// O = sum p V; m is the row's maximum so far, moved only when the maximum has grown by more than kSlack, so that O and l are rescaled a
+// few times per row, not at every block (p stays below 2^kSlack, far inside fp16's range; O / l does not depend on m).
+//
+//  S = Q K^T    tcgen05.mma, both operands in shared memory       [128 rows x 128 positions], fp32 in tensor memory
+//  P            one thread per row reads S, writes P in the cache's type over S
+//  O += P V     tcgen05.mma, P from tensor memory, V from shared memory as it lies in the pages (positions are its K axis)
+//
+// Bound: the tensor core and the exponentials, about even: a block of 128 x 128 x 128 is 1024 cycles of each per SM.  So two
+// tiles of 128 rows (a pair) share the staged keys and values of a thread block and take turns: while one tile's softmax runs
+// the tensor core works for the other.
+//  * Warp 0 loads (TMA; a page's rows of a kv head are a box), warp 1 issues the multiplications, warps 4..7 and 8..11 are the
+//    softmax of the two tiles.  K and V blocks go through one ring of stages.
+//  * The work is cut into equal shares whatever the lengths (lw_attend_plan.h); a pair that is cut leaves unnormalised partial
+//    results, which k_attend_join adds up.  Lengths are read on the device.
+//  * Values of positions that no row of the pair sees are zeroed in shared memory before they are multiplied (a weight of 0
+//    would not hide a NaN that an earlier owner of the page left).
+//  * Rounding: S, m, l, O in 32 bits; P in the cache's type, as the tensor core takes it (half a step of its 11 or 8 bits,
+//    independent from position to position); l adds the unrounded p.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "lw_attend.cuh"
+#include "lw_attend_plan.h"
+#include "lw_tcgen05.cuh"
+
+namespace lw {
+
+constexpr int kPromptThreads = 12 * 32;
+constexpr float kSlack = 8.f;
+
+// What a block left of the pair that its share begins in the middle of (piece 0), or of the one that its share does not finish
+// (piece 1): `begins` and `ends` tell whether piece 0 holds the pair's first and last unit.
+struct PieceNote {
+  int row0, rows, head0, begins, ends;   // first row of the packed queries, rows (tokens), first query head
+  int pad[3];
+};
+
+struct PromptArgs {
+  AttendArgs a;
+  int group, tile_tokens;   // query heads per kv head; tokens of a tile: 128 / group
+  int box_rows;             // positions of a K / V box: a divisor of the page size and of 128
+  int dim16;                // head_dim rounded up to 16
+  int cap;                  // positions the table can name
+  uint32_t wait_limit;
+  PieceNote* notes;         // [gridDim.x]
+  float* partial;           // [gridDim.x][piece][tile]: m[128], l[128], O [dim16 / 4][128][4]
+};
+__host__ __device__ constexpr size_t tile_partial_floats(int dim16) { return 256 + static_cast<size_t>(dim16) * 128; }
+
+struct SeqRows {
+  PromptSeq q;
+  int row0;
+};
+__device__ __forceinline__ SeqRows seq_rows(const PromptArgs& P, int b) {
+  const Sequences& s = P.a.seq;
+  const int r0 = min(max(s.starts[b], 0), P.a.rows), r1 = min(max(s.starts[b + 1], r0), P.a.rows);
+  SeqRows r;
+  r.q.rows = r1 - r0;
+  r.q.len = min(max(s.lens[b], 0), P.cap);
+  r.row0 = r0;
+  return r;
+}
+
+// A run of units of one pair, and the walk over a block's share.  Every role of the block walks by itself.
+struct Walk {
+  int b, h, i, off;
+  long long left;
+  SeqRows s;
+};
+struct Piece {
+  int h, t0, j0, j1;    // kv head, first token of the pair, position blocks
+  bool begins, ends;
+  SeqRows s;
+  int b;
+};
+__device__ __forceinline__ Piece next_piece(const PromptArgs& P, const PromptShape& shape, Walk& w) {
+  const PairRange r = pair_range(shape, w.s.q, w.i);
+  const int n = r.last - r.first, take = static_cast<int>(min(static_cast<long long>(n - w.off), w.left));
+  Piece p;
+  p.h = w.h;
+  p.t0 = w.i * shape.pair_tokens;
+  p.j0 = r.first + w.off;
+  p.j1 = p.j0 + take;
+  p.begins = w.off == 0;
+  p.ends = w.off + take == n;
+  p.s = w.s;
+  p.b = w.b;
+  w.left -= take;
+  if (!p.ends) {
+    w.off += take;
+  } else {
+    w.off = 0;
+    if (++w.i == prompt_pairs(shape, w.s.q)) {
+      w.i = 0;
+      if (++w.h == P.a.pool.Hk) {
+        w.h = 0;
+        if (w.left > 0) {
+          do ++w.b; while (w.b < P.a.seq.n - 1 && seq_rows(P, w.b).q.rows == 0);
+          w.s = seq_rows(P, w.b);
+        }
+      }
+    }
+  }
+  return p;
+}
+
+// One tile of the pair inside a piece: its position blocks there (none: first >= last) and what its rows see.
+struct TileRange {
+  int first, last, p_first, p_last, tokens;   // p_first, p_last: positions of its first and last token
+  __device__ __forceinline__ bool none() const { return first >= last; }
+  __device__ __forceinline__ bool has(int j) const { return j >= first && j < last; }
+};
+__device__ __forceinline__ TileRange tile_range(const PromptArgs& P, const Piece& p, int x) {
+  const int t0 = p.t0 + x * P.tile_tokens, p0 = p.s.q.len - p.s.q.rows;
+  TileRange r;
+  r.tokens = min(P.tile_tokens, p.s.q.rows - t0);
+  r.p_first = p0 + t0;
+  r.p_last = p0 + t0 + r.tokens - 1;
+  const int lo = P.a.window > 0 ? max(0, r.p_first - P.a.window + 1) : 0;
+  r.first = max(p.j0, lo / kPosBlock);
+  r.last = min(p.j1, (r.p_last + kPosBlock) / kPosBlock);
+  if (r.tokens <= 0 || r.p_last < 0) r.last = r.first = 0;
+  return r;
+}
+
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+        "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
+        "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+template <int DP>
+struct PromptSizes {
+  static constexpr uint32_t kTile = 128 * DP * 2;                   // bytes of a tile of queries, a block of keys or of values
+  static constexpr int kStages = DP == 128 ? 5 : 8;
+  static constexpr size_t kSmem = 1024 + 2 * kTile + kStages * kTile;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    k_attend_prompt(const __grid_constant__ CUtensorMap QM, const __grid_constant__ CUtensorMap KM, const __grid_constant__ CUtensorMap VM,
+                    const __grid_constant__ PromptArgs P) {
+  using Z = PromptSizes<DP>;
+  constexpr int kStages = Z::kStages;
+  constexpr uint32_t kHalf = 128 * 128;   // bytes of 64 columns of a tile: 128 rows of 128 bytes, swizzled
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], tail_full, mma_done;
+  __shared__ uint32_t tmem_slot[1];
+  __shared__ int abort_word, s_first[4];
+  __shared__ long long s_scan[kPromptThreads / 32 + 1], s_rest;
+  volatile int* abort_flag = &abort_word;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u, ring = base + 2 * Z::kTile;
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(smem_addr(full + i), 1);
+      mbar_init(smem_addr(empty + i), 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(smem_addr(q_full + x), 1);
+      mbar_init(smem_addr(q_empty + x), 1);
+      mbar_init(smem_addr(s_full + x), 1);
+      mbar_init(smem_addr(p_full + x), 4);
+      mbar_init(smem_addr(o_full + x), 1);
+    }
+    mbar_init(smem_addr(&tail_full), 1);
+    mbar_init(smem_addr(&mma_done), 1);
+    abort_word = 0;
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot[0];
+  pdl_trigger();
+  pdl_wait();
+
+  // ---- this block's share of the units
+  const PromptShape shape = {2 * P.tile_tokens, P.a.window};
+  const int n_seqs = P.a.seq.n;
+  auto seq_units = [&](int b) -> long long {
+    if (b >= n_seqs) return 0;
+    const SeqRows s = seq_rows(P, b);
+    if (blockIdx.x == 0 && P.a.seq.lens[b] > P.cap) atomicOr(P.a.err, kErrWordIndex);
+    return s.q.rows > 0 ? P.a.pool.Hk * units_before(shape, s.q, prompt_pairs(shape, s.q)) : 0;
+  };
+  auto block_sum = [&](long long v, long long& before) -> long long {   // of all threads; before: of the threads in front of this one
+    long long inc = v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long w = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += w;
+    }
+    if (lane == 31) s_scan[warp] = inc;
+    __syncthreads();
+    long long front = 0, all = 0;
+    for (int k = 0; k < kPromptThreads / 32; ++k) {
+      if (k < warp) front += s_scan[k];
+      all += s_scan[k];
+    }
+    __syncthreads();
+    before = front + inc - v;
+    return all;
+  };
+  long long units = 0, dummy;
+  for (int b0 = 0; b0 < n_seqs; b0 += kPromptThreads) units += block_sum(seq_units(b0 + tid), dummy);
+  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), units));   // the others have nothing to do
+  const long long u0 = static_cast<int>(blockIdx.x) < blocks ? share(units, blockIdx.x, blocks) : 0, u1 = static_cast<int>(blockIdx.x) < blocks ? share(units, blockIdx.x + 1, blocks) : 0;
+  if (u0 < u1) {
+    long long front = 0;
+    for (int b0 = 0; b0 < n_seqs; b0 += kPromptThreads) {
+      const long long mine = seq_units(b0 + tid);
+      long long before;
+      const long long all = block_sum(mine, before);
+      if (u0 >= front + before && u0 < front + before + mine) {
+        const SeqRows s = seq_rows(P, b0 + tid);
+        const long long per_head = mine / P.a.pool.Hk, rest = u0 - front - before;
+        s_first[0] = b0 + tid;
+        s_first[1] = static_cast<int>(rest / per_head);
+        s_rest = rest % per_head;
+      }
+      front += all;
+    }
+    __syncthreads();
+    if (warp == 0) {   // the pair that holds unit s_rest of its head: 32-fold search
+      const SeqRows s = seq_rows(P, s_first[0]);
+      int lo = 0, hi = prompt_pairs(shape, s.q);   // units_before(lo) <= s_rest < units_before(hi)
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = min(lo + lane * step, hi);
+        const unsigned int ok = __ballot_sync(0xffffffffu, at < hi && units_before(shape, s.q, at) <= s_rest);
+        const int best = 31 - __clz(ok);           // lane 0 always says yes
+        lo += best * step;
+        hi = min(lo + step, hi);
+      }
+      if (lane == 0) {
+        s_first[2] = lo;
+        s_first[3] = static_cast<int>(s_rest - units_before(shape, s.q, lo));
+      }
+    }
+    __syncthreads();
+  } else if (tid == 0) {
+    P.notes[blockIdx.x] = {0, 0, 0, 1, 1, {0, 0, 0}};
+  }
+  Walk walk = {};
+  walk.left = u1 - u0;
+  if (walk.left > 0) {
+    walk.b = s_first[0];
+    walk.h = s_first[1];
+    walk.i = s_first[2];
+    walk.off = s_first[3];
+    walk.s = seq_rows(P, walk.b);
+  }
+
+  if (warp == 0) {   // ---------------------------------------------------------------- loads
+    int s = 0, q_count[2] = {0, 0}, tails = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    const int per_block = kPosBlock / P.box_rows, halves = DP / 64, n_boxes = per_block * halves;
+    while (walk.left > 0 && ok) {
+      const Piece p = next_piece(P, shape, walk);
+      const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
+      for (int x = 0; x < 2 && ok; ++x) {
+        if (r[x].none()) continue;
+        if (!(ok = t5_wait_warp(q_empty + x, (q_count[x] & 1) ^ 1, P.wait_limit, P.a.err, abort_flag))) break;
+        ++q_count[x];
+        if (lane == 0) {
+          mbar_expect(q_full + x, halves * 128u * P.group * P.tile_tokens);
+          for (int d = 0; d < halves; ++d)
+            tma_load_3d(base + x * Z::kTile + d * kHalf, &QM, 64 * d, p.h * P.group, p.s.row0 + p.t0 + x * P.tile_tokens, smem_addr(q_full + x));
+        }
+      }
+      // positions that some row of the pair sees
+      const PairRange pr = pair_range(shape, p.s.q, p.t0 / shape.pair_tokens);
+      const int* table = P.a.seq.table + p.b * P.a.seq.table_stride;
+      for (int j = p.j0; j < p.j1 && ok; ++j) {
+        if (!r[0].has(j) && !r[1].has(j)) continue;
+        const int end = min(kPosBlock, pr.hi - j * kPosBlock), begin = max(0, pr.lo - j * kPosBlock);
+        const int rows_end = (end + P.box_rows - 1) / P.box_rows, rows_begin = begin / P.box_rows, count = (rows_end - rows_begin) * halves;
+        // lane n < n_boxes: box n % per_block of half n / per_block
+        int page = 0, in_page = 0;
+        const int at = lane % per_block;
+        const bool mine = lane < n_boxes && at >= rows_begin && at < rows_end;
+        if (mine) {
+          const int pos = j * kPosBlock + at * P.box_rows, column = pos / P.a.pool.page_size;
+          page = table[column];
+          in_page = pos - column * P.a.pool.page_size;
+          if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(P.a.pool.n_pages)) {   // the tensor map's bounds fill it with zeros
+            atomicOr(P.a.err, kErrWordIndex);
+            page = P.a.pool.n_pages;
+          }
+        }
+        for (int kv = 0; kv < 2 && ok; ++kv) {
+          if (!(ok = t5_wait_warp(empty + s, ph ^ 1u, P.wait_limit, P.a.err, abort_flag))) break;
+          const uint32_t stage = ring + s * Z::kTile;
+          const bool cut = kv == 1 && (end < kPosBlock || begin > 0);
+          uint64_t* bar = cut ? &tail_full : full + s;
+          if (lane == 0) mbar_expect(bar, count * P.box_rows * 128u);
+          __syncwarp();
+          for (int n = lane; n < n_boxes; n += 32) {   // at most 32 boxes: box_rows is at least 8, halves at most 2
+            if (mine) tma_load_4d(stage + (n / per_block) * kHalf + at * P.box_rows * 128, kv ? &VM : &KM, 64 * (n / per_block), in_page, p.h, page, smem_addr(bar));
+          }
+          if (cut) {
+            ok = t5_wait_warp(&tail_full, tails++ & 1, P.wait_limit, P.a.err, abort_flag);
+            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+            uint8_t* dst = smem_raw + (stage - smem_addr(smem_raw));
+            for (int n = lane; n < kPosBlock * halves * 8; n += 32) {
+              const int row = (n >> 3) & 127, half = n >> 10;
+              if (row >= end || row < begin) *reinterpret_cast<uint4*>(dst + half * kHalf + row * 128 + (n & 7) * 16) = zero;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + s);
+          }
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+    // copies still in flight land before the block gives its shared memory back
+    if (lane == 0) {
+      for (int i = 0; i < kStages; ++i) mbar_wait(smem_addr(full + i), i < s ? ph : ph ^ 1u, P.a.err, 1u << 16);
+      for (int x = 0; x < 2; ++x)
+        if (q_count[x]) mbar_wait(smem_addr(q_full + x), (q_count[x] & 1) ^ 1, P.a.err, 1u << 16);
+    }
+    __syncwarp();
+  } else if (warp == 1) {   // ----------------------------------------------------------- multiplications
+    if (lane == 0) {
+      constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
+      const uint32_t idesc_s = idesc_f16_m128(kPosBlock) | type, idesc_o = idesc_f16_m128(P.dim16) | type | (1u << 16);   // bit 16: V is position-major
+      const int steps = P.dim16 / 16;
+      int s = 0, q_count[2] = {0, 0}, p_count[2] = {0, 0};
+      uint32_t ph = 0;
+      bool ok = true;
+      auto take = [&](uint32_t& stage) -> bool {   // the next stage of the ring
+        if (!t5_wait(full + s, ph, P.wait_limit, P.a.err, abort_flag)) return false;
+        stage = s;
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1u;
+        }
+        return true;
+      };
+      auto scores = [&](int x, uint32_t stage, bool last) {
+        tc_fence_after();
+        const uint64_t q = smem_desc_sw128(base + x * Z::kTile), k = smem_desc_sw128(ring + stage * Z::kTile);
+        for (int i = 0; i < steps; ++i) {   // 32 bytes further inside the swizzle row; then the other half
+          const uint32_t off = (i & 3) * 2 + (i >> 2) * (kHalf >> 4);
+          mma_ss_f16(tmem + x * 128, q + off, k + off, idesc_s, i > 0);
+        }
+        mma_commit(s_full + x);
+        if (last) mma_commit(q_empty + x);
+      };
+      while (walk.left > 0 && ok) {
+        const Piece p = next_piece(P, shape, walk);
+        const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
+        int j = p.j0;
+        while (j < p.j1 && !r[0].has(j) && !r[1].has(j)) ++j;
+        uint32_t k_stage = 0, v_stage = 0;
+        bool more = j < p.j1;
+        if (more) {   // the first scores
+          if (!(ok = take(k_stage))) break;
+          for (int x = 0; x < 2 && ok; ++x)
+            if (r[x].has(j)) {
+              if (!(ok = t5_wait(q_full + x, q_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+              scores(x, k_stage, j + 1 == r[x].last);
+            }
+          mma_commit(empty + k_stage);
+        }
+        for (; more && ok; ++j) {
+          more = j + 1 < p.j1 && (r[0].has(j + 1) || r[1].has(j + 1));
+          if (!(ok = take(v_stage)) || (more && !(ok = take(k_stage)))) break;
+          const uint64_t v = (smem_desc_sw128(ring + v_stage * Z::kTile) & ~(0x3FFFull << 16)) | (static_cast<uint64_t>(kHalf >> 4) << 16);
+          for (int x = 0; x < 2 && ok; ++x) {
+            if (r[x].has(j)) {
+              if (!(ok = t5_wait(p_full + x, p_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+              tc_fence_after();
+              for (int i = 0; i < 8; ++i)   // 16 positions further: two groups of eight rows
+                mma_ts_f16(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, v + i * (2048 >> 4), idesc_o, j > r[x].first || i > 0);
+              if (j + 1 == r[x].last) mma_commit(o_full + x);
+            }
+            if (more && r[x].has(j + 1)) {
+              if (j + 1 == r[x].first && !(ok = t5_wait(q_full + x, q_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+              scores(x, k_stage, j + 2 == r[x].last);
+            }
+          }
+          mma_commit(empty + v_stage);
+          if (more) mma_commit(empty + k_stage);
+        }
+      }
+      mma_commit(&mma_done);   // they read shared memory and write tensor memory, which the block is about to give back
+      mbar_wait(smem_addr(&mma_done), 0, P.a.err, 1u << 16);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {   // -------------------------------------------------------------- softmax
+    const int x = (warp >> 2) - 1, row = (warp & 3) * 32 + lane, token = row / P.group, head = row - token * P.group;
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t ts = tmem + lanes + x * 128, to = tmem + lanes + 256 + x * 128;
+    const bool flip = P.a.scale < 0.f;
+    // a scale of 0 becomes a very small one: a score hidden as -inf must stay -inf
+    const float c = fmaxf(fabsf(P.a.scale) * 1.4426950408889634f, 1e-30f);
+    int s_count = 0, o_count = 0;
+    bool ok = true, first = true;
+    while (walk.left > 0 && ok) {
+      const Piece p = next_piece(P, shape, walk);
+      const TileRange r = tile_range(P, p, x);
+      const bool mine = token < min(r.tokens, P.tile_tokens);
+      const int pos = mine ? r.p_first + token : -1;
+      const int lo = P.a.window > 0 ? max(0, pos - P.a.window + 1) : 0;
+      const bool idle = !__any_sync(0xffffffffu, mine);
+      float m = -INFINITY, l = 0.f;
+      for (int j = r.first; j < r.last; ++j) {
+        if (!(ok = t5_wait_warp(s_full + x, s_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+        if (!idle) {
+          tc_fence_after();
+          uint32_t v[128];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tmem_load32(ts + 32 * k, v + 32 * k);
+          tmem_wait_load();
+          if (flip) {
+#pragma unroll
+            for (int k = 0; k < 128; ++k) v[k] ^= 0x80000000u;
+          }
+          const int p0 = j * kPosBlock;
+          if (p0 + kPosBlock - 1 > r.p_first || (P.a.window > 0 && p0 <= r.p_last - P.a.window)) {   // some row does not see all of it
+            const int top = pos - p0, bottom = lo - p0;
+#pragma unroll
+            for (int k = 0; k < 128; ++k)
+              if (k > top || k < bottom) v[k] = 0xff800000u;
+          }
+          float mx = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 128; ++k) mx = fmaxf(mx, __uint_as_float(v[k]));
+          mx *= c;
+          const bool grow = mx > m + kSlack;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float m2 = grow ? mx : m, keep = m == -INFINITY ? 0.f : exp2_fast(m - m2);   // nothing seen yet: O and l count for nothing
+            m = m2;
+            l *= keep;
+            if (j > r.first) {   // PV of the block before is done: its completion came with these scores
+#pragma unroll 1
+              for (int d = 0; d < P.dim16; d += 16) {
+                uint32_t o[16];
+                tmem_load16(to + d, o);
+                tmem_wait_load();
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(keep == 0.f ? 0.f : __uint_as_float(o[k]) * keep);
+                tmem_store16(to + d, o);
+              }
+            }
+          }
+          const float ref = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            uint32_t h[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float e0 = exp2_fast(fmaf(__uint_as_float(v[16 * k + 2 * i]), c, -ref)), e1 = exp2_fast(fmaf(__uint_as_float(v[16 * k + 2 * i + 1]), c, -ref));
+              sum[(2 * i) & 3] += e0;
+              sum[(2 * i + 1) & 3] += e1;
+              h[i] = pack2<T>(e0, e1);
+            }
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(ts + 8 * k), "r"(h[0]), "r"(h[1]), "r"(h[2]),
+                         "r"(h[3]), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7])
+                         : "memory");
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_store();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + x);
+      }
+      if (!ok) break;
+      if (!r.none() && !(ok = t5_wait_warp(o_full + x, o_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+      tc_fence_after();
+      if (p.begins && p.ends) {
+        if (!idle) {
+          const float f = 1.f / l;   // 0 only if the row sees nothing
+          T* out = static_cast<T*>(P.a.out) + static_cast<long long>(p.s.row0 + p.t0 + x * P.tile_tokens + token) * P.a.out_token +
+                   static_cast<long long>(p.h * P.group + head) * P.a.out_head;
+          for (int d = 0; d < P.dim16; d += 16) {
+            uint32_t o[16];
+            if (!r.none()) {
+              tmem_load16(to + d, o);
+              tmem_wait_load();
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              o[k] = pos < 0 || r.none() ? 0u : __float_as_uint(__uint_as_float(o[k]) * f);
+            if (mine) {
+              auto half8 = [&](int k) { return make_uint4(pack2<T>(__uint_as_float(o[k]), __uint_as_float(o[k + 1])), pack2<T>(__uint_as_float(o[k + 2]), __uint_as_float(o[k + 3])),
+                                                          pack2<T>(__uint_as_float(o[k + 4]), __uint_as_float(o[k + 5])), pack2<T>(__uint_as_float(o[k + 6]), __uint_as_float(o[k + 7]))); };
+              *reinterpret_cast<uint4*>(out + d) = half8(0);
+              if (d + 8 < P.a.pool.Dh) *reinterpret_cast<uint4*>(out + d + 8) = half8(8);
+            }
+          }
+        }
+      } else if (!idle) {
+        float* part = P.partial + (static_cast<size_t>(blockIdx.x) * 4 + (p.begins ? 2 : 0) + x) * tile_partial_floats(P.dim16);
+        part[row] = pos < 0 ? -INFINITY : m;
+        part[128 + row] = pos < 0 ? 0.f : l;
+        if (!r.none()) {
+          for (int d = 0; d < P.dim16; d += 16) {
+            uint32_t o[16];
+            tmem_load16(to + d, o);
+            tmem_wait_load();
+#pragma unroll
+            for (int k = 0; k < 16; k += 4)
+              *reinterpret_cast<uint4*>(part + 256 + (static_cast<size_t>((d + k) / 4) * 128 + row) * 4) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          }
+        }
+      }
+      tc_fence_before();   // the next P is announced after these reads of O
+      if (first && x == 0 && (warp & 3) == 0 && lane == 0)
+        P.notes[blockIdx.x] = {p.s.row0 + p.t0, min(2 * P.tile_tokens, p.s.q.rows - p.t0), p.h * P.group, p.begins, p.ends, {0, 0, 0}};
+      first = false;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Pairs that were cut: block (c, y) joins 32 of the rows of the pair that block c of the attention kernel continued, if it is the first
+// to continue it.  O = sum_k 2^(m_k - m) O_k / sum_k 2^(m_k - m) l_k over the pieces in order.
+constexpr int kJoinThreads = 128;
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_constant__ PromptArgs P, int blocks) {
+  pdl_trigger();
+  pdl_wait();
+  const int c = blockIdx.x + 1, x = blockIdx.y >> 2, row = (blockIdx.y & 3) * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
+  // ordinary loads through a volatile-free pointer: the notes were written by the kernel before
+  const PieceNote n = P.notes[c];
+  if (n.begins) return;
+  const PieceNote before = P.notes[c - 1];
+  if (!before.begins && !before.ends) return;   // that block is not the first either
+  const int token = row / P.group, head = row - token * P.group, t = x * P.tile_tokens + token;
+  if (token >= P.tile_tokens || t >= n.rows) return;
+  int last = c;
+  while (!P.notes[last].ends && last + 1 < blocks) ++last;
+  const size_t tile = tile_partial_floats(P.dim16);
+  auto piece = [&](int k) { return P.partial + (static_cast<size_t>(k) * 4 + (k < c ? 2 : 0) + x) * tile; };
+  float m = -INFINITY, l = 0.f;
+  for (int k = c - 1; k <= last; ++k) m = fmaxf(m, piece(k)[row]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int k = c - 1; k <= last; ++k) l += piece(k)[128 + row] * exp2_fast(piece(k)[row] - ref);
+  T* out = static_cast<T*>(P.a.out) + static_cast<long long>(n.row0 + t) * P.a.out_token + static_cast<long long>(n.head0 + head) * P.a.out_head;
+  for (int d = warp * 4; d < P.a.pool.Dh; d += kJoinThreads / 32 * 4) {
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = c - 1; k <= last; ++k) {
+      const float* part = piece(k);
+      if (part[128 + row] == 0.f) continue;   // the piece holds nothing for this row, and no O
+      const float f = exp2_fast(part[row] - ref);
+      const float4 v = *reinterpret_cast<const float4*>(part + 256 + (static_cast<size_t>(d / 4) * 128 + row) * 4);
+      o.x = fmaf(f, v.x, o.x);
+      o.y = fmaf(f, v.y, o.y);
+      o.z = fmaf(f, v.z, o.z);
+      o.w = fmaf(f, v.w, o.w);
+    }
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(o.x * f, o.y * f), pack2<T>(o.z * f, o.w * f));
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------- launch
+
+static size_t notes_bytes(int blocks) { return (static_cast<size_t>(blocks) * sizeof(PieceNote) + 255) / 256 * 256; }
+
+long long prompt_workspace(int head_dim) {
+  const int dim16 = (head_dim + 15) / 16 * 16, blocks = sm_count();
+  return static_cast<long long>(notes_bytes(blocks) + static_cast<size_t>(blocks) * 4 * tile_partial_floats(dim16) * sizeof(float));
+}
+
+template <typename T, int DP>
+static int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const PromptArgs& p, cudaStream_t st) {
+  static bool configured_per_device[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  bool& configured = configured_per_device[dev & 63];
+  if (!configured) {
+    if (cudaFuncSetAttribute(k_attend_prompt<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PromptSizes<DP>::kSmem)) != cudaSuccess)
+      return note_launch("cudaFuncSetAttribute(k_attend_prompt)");
+    configured = true;
+  }
+  const int blocks = sm_count();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kPromptThreads);
+  cfg.dynamicSmemBytes = PromptSizes<DP>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, k_attend_prompt<T, DP>, qm, km, vm, p);
+  if (const int rc = note_launch("k_attend_prompt")) return rc;
+  if (blocks < 2) return kOk;
+  cfg.gridDim = dim3(blocks - 1, 8);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
+  cudaLaunchKernelEx(&cfg, k_attend_join<T>, p, blocks);
+  return note_launch("k_attend_join");
+}
+
+int launch_attend_prompt(const PagedCache& cache, const AttendArgs& a, cudaStream_t st) {
+  PromptArgs p = {};
+  p.a = a;
+  p.group = a.H / a.pool.Hk;
+  p.tile_tokens = 128 / p.group;
+  p.box_rows = std::min(kPosBlock, a.pool.page_size & -a.pool.page_size);
+  p.dim16 = (a.pool.Dh + 15) / 16 * 16;
+  p.cap = static_cast<int>(std::min<long long>(static_cast<long long>(a.seq.table_cols) * a.pool.page_size, 1 << 30));
+  p.wait_limit = debug_knobs().wait_limit;
+  p.notes = static_cast<PieceNote*>(a.workspace);
+  p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + notes_bytes(sm_count()));
+  alignas(64) CUtensorMap qm, km, vm;
+  const bool half = cache.type == kF16;
+  if (!make_query_map(&qm, half, a.q, a.pool.Dh, a.H, a.rows, a.q_head, a.q_token, p.group, p.tile_tokens) ||
+      !make_page_map(&km, half, a.pool.k, a.pool, p.box_rows) || !make_page_map(&vm, half, a.pool.v, a.pool, p.box_rows)) {
+    set_kernel_error_text("attend_prompt", "the driver refused a tensor map over the queries or the pages");
+    return kErrArg;
+  }
+  if (a.pool.Dh <= 64) return half ? launch<__half, 64>(qm, km, vm, p, st) : launch<__nv_bfloat16, 64>(qm, km, vm, p, st);
+  return half ? launch<__half, 128>(qm, km, vm, p, st) : launch<__nv_bfloat16, 128>(qm, km, vm, p, st);
+}
+
+}  // namespace lw

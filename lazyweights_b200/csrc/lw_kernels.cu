@@ -23,6 +23,7 @@
 
 #include "lw_ring.cuh"
 #include "lw_gemv1.h"
+#include "lw_paged.h"
 
 namespace lw {
 
@@ -368,6 +369,31 @@ bool make_half_slab_map(void* tensor_map, const void* base, size_t K, size_t row
   const cuuint32_t estr[2] = {1, 1};
   return encode(static_cast<CUtensorMap*>(tensor_map), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool make_query_map(void* tensor_map, bool half, const void* base, int Dh, int H, int rows, long long head_stride, long long token_stride,
+                    int box_heads, int box_tokens) {
+  const PFN_cuTensorMapEncodeTiled encode = tensor_map_encoder();
+  if (!encode) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(Dh), static_cast<cuuint64_t>(H), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_stride) * 2, static_cast<cuuint64_t>(token_stride) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return encode(static_cast<CUtensorMap*>(tensor_map), half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool make_page_map(void* tensor_map, bool half, const void* base, const PagePool& p, int box_rows) {
+  const PFN_cuTensorMapEncodeTiled encode = tensor_map_encoder();
+  if (!encode) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.Dh), static_cast<cuuint64_t>(p.page_size), static_cast<cuuint64_t>(p.Hk), static_cast<cuuint64_t>(p.n_pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(p.token_stride) * 2, static_cast<cuuint64_t>(p.head_stride) * 2, static_cast<cuuint64_t>(p.page_stride) * 2};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return encode(static_cast<CUtensorMap*>(tensor_map), half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // SMs of the current device (cached per device: a process may hold handles on several).

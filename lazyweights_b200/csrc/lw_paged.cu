@@ -317,6 +317,7 @@ static int attend(const char* what, void* cache, const void* q, long long q_toke
   if (const int rc = check_sequences(what, starts, lens, table, n_seqs, table_cols, table_stride, n_rows, prompt)) return rc;
   if (const int rc = check_rows(what, q, q_token_stride, q_head_stride, n_heads, c->pool.Dh, n_rows)) return rc;
   if (const int rc = check_rows(what, out, out_token_stride, out_head_stride, n_heads, c->pool.Dh, n_rows)) return rc;
+  if (n_heads / c->pool.Hk > 128) return refuse(what, "at most 128 query heads per kv head");
   if (!std::isfinite(scale) || window < 0) return refuse(what, "the scale must be finite, the window not negative");
   const long long need = lw_cache_workspace(cache, n_rows, n_heads, prompt);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
@@ -337,14 +338,13 @@ static int attend(const char* what, void* cache, const void* q, long long q_toke
   a.scale = scale;
   a.workspace = workspace;
   if (!(a.err = error_word())) return cuda_fail("error word", cudaGetLastError());
-  return launch_attend(c->type, a, static_cast<cudaStream_t>(stream));
+  return prompt ? launch_attend_prompt(*c, a, static_cast<cudaStream_t>(stream)) : launch_attend(c->type, a, static_cast<cudaStream_t>(stream));
 }
 
 long long lw_cache_workspace(void* cache, int n_rows, int n_heads, int prompt) {
   const PagedCache* c = static_cast<const PagedCache*>(cache);
   if (!c || n_rows < 1 || n_heads < 1 || n_heads % c->pool.Hk) return refuse("lw_cache_workspace", "bad argument");
-  (void)prompt;
-  return 0;
+  return prompt ? prompt_workspace(c->pool.Dh) : 0;
 }
 
 int lw_cache_attend(void* cache, const void* q, long long q_token_stride, long long q_head_stride, int n_seqs, int n_heads, const int* lens,

@@ -50,4 +50,14 @@ struct AttendArgs {
 
 int launch_attend(ElemType type, const AttendArgs& a, cudaStream_t st);
 
+// Prompts (lw_attend_prompt.cu); the workspace that any of them needs on the current device.
+int launch_attend_prompt(const PagedCache& cache, const AttendArgs& a, cudaStream_t st);
+long long prompt_workspace(int head_dim);
+
+// Tensor maps in the 128-byte swizzle (boxes of 64 columns): queries [rows][H][Dh], boxes of box_tokens x box_heads rows; pages,
+// boxes of box_rows positions of one head.  False where the driver does not offer the encoder or refuses the shape.
+bool make_query_map(void* tensor_map, bool half, const void* base, int Dh, int H, int rows, long long head_stride, long long token_stride,
+                    int box_heads, int box_tokens);
+bool make_page_map(void* tensor_map, bool half, const void* base, const PagePool& pool, int box_rows);
+
 }  // namespace lw
