@@ -338,13 +338,13 @@ static int attend(const char* what, void* cache, const void* q, long long q_toke
   a.scale = scale;
   a.workspace = workspace;
   if (!(a.err = error_word())) return cuda_fail("error word", cudaGetLastError());
-  return prompt ? launch_attend_prompt(*c, a, static_cast<cudaStream_t>(stream)) : launch_attend(c->type, a, static_cast<cudaStream_t>(stream));
+  return (prompt ? launch_attend_prompt : launch_attend_token)(*c, a, static_cast<cudaStream_t>(stream));
 }
 
 long long lw_cache_workspace(void* cache, int n_rows, int n_heads, int prompt) {
   const PagedCache* c = static_cast<const PagedCache*>(cache);
   if (!c || n_rows < 1 || n_heads < 1 || n_heads % c->pool.Hk) return refuse("lw_cache_workspace", "bad argument");
-  return prompt ? prompt_workspace(c->pool.Dh) : 0;
+  return prompt ? prompt_workspace(c->pool.Dh) : token_workspace(c->pool.Dh, n_heads / c->pool.Hk);
 }
 
 int lw_cache_attend(void* cache, const void* q, long long q_token_stride, long long q_head_stride, int n_seqs, int n_heads, const int* lens,

@@ -1,5 +1,5 @@
 // The paged key-value cache: geometry handle, launchers of the kernels that fill and read it (lw_paged.cu: appending with
-// the position rotation, C ABI; lw_attend.cuh / .cu: attention).
+// the position rotation, C ABI; lw_attend_token.cu, lw_attend_prompt.cu: attention).
 #pragma once
 #include <cuda.h>
 
@@ -48,9 +48,10 @@ struct AttendArgs {
   unsigned int* err;
 };
 
-int launch_attend(ElemType type, const AttendArgs& a, cudaStream_t st);
-
-// Prompts (lw_attend_prompt.cu); the workspace that any of them needs on the current device.
+// One token per sequence (lw_attend_token.cu) and packed prompts (lw_attend_prompt.cu); the workspace that calls of any size
+// need on the current device.
+int launch_attend_token(const PagedCache& cache, const AttendArgs& a, cudaStream_t st);
+long long token_workspace(int head_dim, int group);
 int launch_attend_prompt(const PagedCache& cache, const AttendArgs& a, cudaStream_t st);
 long long prompt_workspace(int head_dim);
 
