@@ -34,10 +34,10 @@ namespace lw {
 constexpr int kPromptThreads = 12 * 32;
 constexpr float kSlack = 8.f;
 
-// What a block left of the pair that its share begins in the middle of (piece 0), or of the one that its share does not finish
-// (piece 1): `begins` and `ends` tell whether piece 0 holds the pair's first and last unit.
+// The pair that block c continues: its first packed row, rows (tokens) and first query head, and the blocks that hold its first and
+// last unit (first == c: none).  A block leaves the pair that it continues as its piece 0, the one that it only begins as piece 1.
 struct PieceNote {
-  int row0, rows, head0, begins, ends;   // first row of the packed queries, rows (tokens), first query head
+  int row0, rows, head0, first, last;
   int pad[3];
 };
 
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     __syncthreads();
   } else if (tid == 0) {
-    P.notes[blockIdx.x] = {0, 0, 0, 1, 1, {0, 0, 0}};
+    P.notes[blockIdx.x] = {0, 0, 0, static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.x), {0, 0, 0}};
   }
   Walk walk = {};
   walk.left = u1 - u0;
@@ -260,6 +260,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     walk.i = s_first[2];
     walk.off = s_first[3];
     walk.s = seq_rows(P, walk.b);
+    if (tid == 0) {
+      const PairRange r = pair_range(shape, walk.s.q, walk.i);
+      const long long begin = u0 - walk.off;   // unit u is block floor(((u + 1) blocks - 1) / units)'s
+      const int t0 = walk.i * shape.pair_tokens, me = blockIdx.x;
+      P.notes[me] = {walk.s.row0 + t0, min(shape.pair_tokens, walk.s.q.rows - t0), walk.h * P.group,
+                     walk.off ? static_cast<int>(((begin + 1) * blocks - 1) / units) : me,
+                     walk.off ? static_cast<int>(((begin + r.last - r.first) * blocks - 1) / units) : me, {0, 0, 0}};
+    }
   }
 
   if (warp == 0) {   // ---------------------------------------------------------------- loads
@@ -412,7 +420,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // a scale of 0 becomes a very small one: a score hidden as -inf must stay -inf
     const float c = fmaxf(fabsf(P.a.scale) * 1.4426950408889634f, 1e-30f);
     int s_count = 0, o_count = 0;
-    bool ok = true, first = true;
+    bool ok = true;
     while (walk.left > 0 && ok) {
       const Piece p = next_piece(P, shape, walk);
       const TileRange r = tile_range(P, p, x);
@@ -525,9 +533,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       }
       tc_fence_before();   // the next P is announced after these reads of O
-      if (first && x == 0 && (warp & 3) == 0 && lane == 0)
-        P.notes[blockIdx.x] = {p.s.row0 + p.t0, min(2 * P.tile_tokens, p.s.q.rows - p.t0), p.h * P.group, p.begins, p.ends, {0, 0, 0}};
-      first = false;
     }
   }
   tc_fence_before();
@@ -542,19 +547,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 // to continue it.  O = sum_k 2^(m_k - m) O_k / sum_k 2^(m_k - m) l_k over the pieces in order.
 constexpr int kJoinThreads = 128;
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_constant__ PromptArgs P, int blocks) {
+__global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_constant__ PromptArgs P) {
   pdl_trigger();
   pdl_wait();
   const int c = blockIdx.x + 1, x = blockIdx.y >> 2, row = (blockIdx.y & 3) * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
-  // ordinary loads through a volatile-free pointer: the notes were written by the kernel before
   const PieceNote n = P.notes[c];
-  if (n.begins) return;
-  const PieceNote before = P.notes[c - 1];
-  if (!before.begins && !before.ends) return;   // that block is not the first either
+  if (n.first != c - 1) return;   // nothing continued, or not the first to continue it
   const int token = row / P.group, head = row - token * P.group, t = x * P.tile_tokens + token;
   if (token >= P.tile_tokens || t >= n.rows) return;
-  int last = c;
-  while (!P.notes[last].ends && last + 1 < blocks) ++last;
+  const int last = n.last;
   const size_t tile = tile_partial_floats(P.dim16);
   auto piece = [&](int k) { return P.partial + (static_cast<size_t>(k) * 4 + (k < c ? 2 : 0) + x) * tile; };
   float m = -INFINITY, l = 0.f;
@@ -616,7 +617,7 @@ static int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMa
   cfg.gridDim = dim3(blocks - 1, 8);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
-  cudaLaunchKernelEx(&cfg, k_attend_join<T>, p, blocks);
+  cudaLaunchKernelEx(&cfg, k_attend_join<T>, p);
   return note_launch("k_attend_join");
 }
 
