@@ -14,9 +14,10 @@
 //  * A warp is a worker of its own, with its own share of the positions, its own ring of stages that its TMA loads fill (192 KB per SM
 //    in flight with eight warps; about 45 KB would cover the latency at full bandwidth), its own m, l, O.  Warps never wait for one
 //    another: a batch of short sequences is a row of small pieces with loads of queries and stores of results between them, and a
-//    block whose warps met at every piece took 146 instead of XX us for 33 sequences of 30 to 4000 positions with 32 kv heads.
-//  * Shares: units of 16 positions of a kv head, numbered sequence by sequence, head by head; every worker takes the same
-//    number, whatever the lengths, which it reads on the device.  What a worker begins or ends in the middle of goes to the workspace
+//    block whose warps met at every piece took 146 instead of 89 us for 33 sequences of 30 to 4000 positions with 32 kv heads.
+//  * Shares: units of 16 positions of a kv head, numbered sequence by sequence, head by head, each sequence and head led by kLead
+//    units that stand for what it costs besides (queries in, results out); every worker takes the same number, whatever the
+//    lengths, which it reads on the device.  What a worker begins or ends in the middle of goes to the workspace
 //    and is joined, in order, by k_token_join.
 //  * Positions outside the sequence or the window: scores replaced by -inf, values zeroed in shared memory (0 x NaN is NaN).
 //  * Rounding: scores, m, l, O in 32 bits, P in the cache's type for the tensor core (half a step of it, independent per position).
@@ -32,6 +33,7 @@ namespace lw {
 constexpr int kTokenWarps = 4, kTokenThreads = kTokenWarps * 32;
 constexpr int kUnit = 16;                 // positions of a unit
 constexpr int kTokenBlocksPerSm = 2;
+constexpr int kLead = 2;                  // see above: 200 sequences of 10 to 500 positions, 8 kv heads: 32.1 us (0: 41.7, 1: 34.5, 4: 32.5)
 
 // The piece that worker w continues: sequence, head slot, the workers that hold its first and last unit (first == w: none).
 struct TokenNote {
@@ -87,7 +89,8 @@ __device__ __forceinline__ TokenSeq token_seq(const TokenArgs& P, int b) {
   return s;
 }
 
-// Where a walk over the block's share stands: unit t of head slot h (kv head, pass) of sequence b.
+// Where a walk over a worker's share stands: unit t of head slot h (kv head, pass) of sequence b; `left` units to go, the leading ones of
+// sequences and heads still to come among them.
 struct TokenWalk {
   int b, h, t;
   long long left;
@@ -95,6 +98,7 @@ struct TokenWalk {
   __device__ __forceinline__ void step(const TokenArgs& P, int slots) {
     --left;
     if (++t < s.last) return;
+    left -= kLead;
     if (++h == slots) {
       h = 0;
       if (left > 0) {
@@ -151,7 +155,7 @@ __global__ void __launch_bounds__(kTokenThreads, kTokenBlocksPerSm)
     if (b >= n_seqs) return 0;
     const TokenSeq s = token_seq(P, b);
     if (blockIdx.x == 0 && P.a.seq.lens[b] > P.cap) atomicOr(P.a.err, kErrWordIndex);
-    return static_cast<long long>(max(0, s.last - s.first)) * slots;
+    return s.last > s.first ? static_cast<long long>(s.last - s.first + kLead) * slots : 0;
   };
   auto block_sum = [&](long long v, long long& before) -> long long {
     long long inc = v;
@@ -184,10 +188,10 @@ __global__ void __launch_bounds__(kTokenThreads, kTokenBlocksPerSm)
         if (worker >= workers) break;
         const long long rest = share(units, worker, workers) - front - before;
         if (rest >= 0 && rest < mine) {
-          const int per_slot = s.last - s.first, slot = static_cast<int>(rest / per_slot);   // int: a pool's positions of one sequence and its heads
+          const int per_slot = s.last - s.first + kLead, slot = static_cast<int>(rest / per_slot);
           s_start[w][0] = b0 + tid;
           s_start[w][1] = slot;
-          s_start[w][2] = s.first + static_cast<int>(rest - static_cast<long long>(slot) * per_slot);
+          s_start[w][2] = s.first - kLead + static_cast<int>(rest - static_cast<long long>(slot) * per_slot);   // below s.first: among the leading units
         }
       }
     }
@@ -202,24 +206,26 @@ __global__ void __launch_bounds__(kTokenThreads, kTokenBlocksPerSm)
   }
   __syncthreads();
   const int worker = warp * gridDim.x + blockIdx.x;
-  if (worker >= workers) {
-    if (lane == 0) P.notes[worker] = {0, 0, worker, worker};
-    return;
+  long long u0 = 0, u1 = 0;
+  TokenWalk at = {};
+  if (worker < workers) {
+    u0 = share(units, worker, workers);
+    u1 = share(units, worker + 1, workers);
+    at.b = s_start[warp][0];
+    at.h = s_start[warp][1];
+    at.s = token_seq(P, at.b);
+    at.t = max(s_start[warp][2], at.s.first);
+    at.left = u1 - u0 - (at.t - s_start[warp][2]);
   }
-  const long long u0 = share(units, worker, workers), u1 = share(units, worker + 1, workers);
-  TokenWalk at;
-  at.b = s_start[warp][0];
-  at.h = s_start[warp][1];
-  at.t = s_start[warp][2];
-  at.left = u1 - u0;
-  at.s = token_seq(P, at.b);
+  // the piece at hand, if it began before: its units are begin .. begin + last - first - 1 of all, unit u is worker
+  // floor(((u + 1) workers - 1) / units)'s
   if (lane == 0) {
-    // the piece at hand holds units begin .. begin + last - first - 1 of all; unit u is worker floor(((u + 1) workers - 1) / units)'s
+    const bool continued = at.left > 0 && at.t > at.s.first;
     const long long begin = u0 - (at.t - at.s.first);
-    const bool continued = at.t > at.s.first;
     P.notes[worker] = {at.b, at.h, continued ? static_cast<int>(((begin + 1) * workers - 1) / units) : worker,
                        continued ? static_cast<int>(((begin + at.s.last - at.s.first) * workers - 1) / units) : worker};
   }
+  if (at.left <= 0) return;
 
   // ---- loads.  Lane n of the first few starts box n of a unit: keys, then values; half by half of the head dimension; 16 positions
   // in one box or two of eight.  The page of the next unit is asked for when the unit before it is started.
@@ -295,6 +301,13 @@ __global__ void __launch_bounds__(kTokenThreads, kTokenBlocksPerSm)
           const int d = k * 16 + e * 8 + (lane & 3) * 2;
           qf[n][k][e] = head < heads && d < P.a.pool.Dh ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
         }
+    }
+    {   // the queries of the next piece, towards the L1 cache
+      const bool same = h + 1 < slots;
+      const int nb = same ? b : b + 1, nh = same ? h + 1 : 0, rows = min(8 * NT, P.group - (nh % P.chunks) * 8 * NT);
+      const int line = lane & 1, head = lane >> 1;
+      if (at.left > t_end - t_begin && nb < n_seqs && head < rows && line * 64 < P.a.pool.Dh)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const T*>(P.a.q) + nb * P.a.q_token + ((nh / P.chunks) * P.group + (nh % P.chunks) * 8 * NT + head) * P.a.q_head + line * 64));
     }
     float m[NT][2], l[NT][2], o[NT][kSteps][4];
 #pragma unroll

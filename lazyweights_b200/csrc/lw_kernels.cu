@@ -384,6 +384,8 @@ bool make_query_map(void* tensor_map, bool half, const void* base, int Dh, int H
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// No promotion of L2 fetches: where the heads lie inside the positions of a page, the neighbouring bytes are another head's (33
+// sequences, 32 kv heads of 96 dimensions: 97 instead of 107 us); where they do not, it makes no difference.
 bool make_page_map(void* tensor_map, bool half, const void* base, const PagePool& p, int box_rows) {
   const PFN_cuTensorMapEncodeTiled encode = tensor_map_encoder();
   if (!encode) return false;
@@ -393,7 +395,7 @@ bool make_page_map(void* tensor_map, bool half, const void* base, const PagePool
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   return encode(static_cast<CUtensorMap*>(tensor_map), half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                 const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // SMs of the current device (cached per device: a process may hold handles on several).
