@@ -32,6 +32,7 @@
 namespace lw {
 
 constexpr int kPromptThreads = 12 * 32;
+constexpr int kPromptRegsSoftmax = 208, kPromptRegsOther = 88;   // 8 and 4 warps: 12 x 168, the launch's
 constexpr float kSlack = 8.f;
 
 // The pair that block c continues: its first packed row, rows (tokens) and first query head, and the blocks that hold its first and
@@ -141,6 +142,28 @@ __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* v) {
       : "memory");
 }
 
+// Two 32-bit operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+// The largest of three; a NaN stays
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 template <int DP>
 struct PromptSizes {
   static constexpr uint32_t kTile = 128 * DP * 2;                   // bytes of a tile of queries, a block of keys or of values
@@ -156,7 +179,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   constexpr int kStages = Z::kStages;
   constexpr uint32_t kHalf = 128 * 128;   // bytes of 64 columns of a tile: 128 rows of 128 bytes, swizzled
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], tail_full, mma_done;
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], tail_full, mma_done;
   __shared__ uint32_t tmem_slot[1];
   __shared__ int abort_word, s_first[4];
   __shared__ long long s_scan[kPromptThreads / 32 + 1], s_rest;
@@ -172,6 +195,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(smem_addr(q_full + x), 1);
       mbar_init(smem_addr(q_empty + x), 1);
       mbar_init(smem_addr(s_full + x), 1);
+      mbar_init(smem_addr(p_half + x), 4);
       mbar_init(smem_addr(p_full + x), 4);
       mbar_init(smem_addr(o_full + x), 1);
     }
@@ -270,149 +294,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   }
 
-  if (warp == 0) {   // ---------------------------------------------------------------- loads
-    int s = 0, q_count[2] = {0, 0}, tails = 0;
-    uint32_t ph = 0;
-    bool ok = true;
-    const int per_block = kPosBlock / P.box_rows, halves = DP / 64, n_boxes = per_block * halves;
-    while (walk.left > 0 && ok) {
-      const Piece p = next_piece(P, shape, walk);
-      const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
-      for (int x = 0; x < 2 && ok; ++x) {
-        if (r[x].none()) continue;
-        if (!(ok = t5_wait_warp(q_empty + x, (q_count[x] & 1) ^ 1, P.wait_limit, P.a.err, abort_flag))) break;
-        ++q_count[x];
-        if (lane == 0) {
-          mbar_expect(q_full + x, halves * 128u * P.group * P.tile_tokens);
-          for (int d = 0; d < halves; ++d)
-            tma_load_3d(base + x * Z::kTile + d * kHalf, &QM, 64 * d, p.h * P.group, p.s.row0 + p.t0 + x * P.tile_tokens, smem_addr(q_full + x));
-        }
-      }
-      // positions that some row of the pair sees
-      const PairRange pr = pair_range(shape, p.s.q, p.t0 / shape.pair_tokens);
-      const int* table = P.a.seq.table + p.b * P.a.seq.table_stride;
-      for (int j = p.j0; j < p.j1 && ok; ++j) {
-        if (!r[0].has(j) && !r[1].has(j)) continue;
-        const int end = min(kPosBlock, pr.hi - j * kPosBlock), begin = max(0, pr.lo - j * kPosBlock);
-        const int rows_end = (end + P.box_rows - 1) / P.box_rows, rows_begin = begin / P.box_rows, count = (rows_end - rows_begin) * halves;
-        // lane n < n_boxes: box n % per_block of half n / per_block
-        int page = 0, in_page = 0;
-        const int at = lane % per_block;
-        const bool mine = lane < n_boxes && at >= rows_begin && at < rows_end;
-        if (mine) {
-          const int pos = j * kPosBlock + at * P.box_rows, column = pos / P.a.pool.page_size;
-          page = table[column];
-          in_page = pos - column * P.a.pool.page_size;
-          if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(P.a.pool.n_pages)) {   // the tensor map's bounds fill it with zeros
-            atomicOr(P.a.err, kErrWordIndex);
-            page = P.a.pool.n_pages;
-          }
-        }
-        for (int kv = 0; kv < 2 && ok; ++kv) {
-          if (!(ok = t5_wait_warp(empty + s, ph ^ 1u, P.wait_limit, P.a.err, abort_flag))) break;
-          const uint32_t stage = ring + s * Z::kTile;
-          const bool cut = kv == 1 && (end < kPosBlock || begin > 0);
-          uint64_t* bar = cut ? &tail_full : full + s;
-          if (lane == 0) mbar_expect(bar, count * P.box_rows * 128u);
-          __syncwarp();
-          for (int n = lane; n < n_boxes; n += 32) {   // at most 32 boxes: box_rows is at least 8, halves at most 2
-            if (mine) tma_load_4d(stage + (n / per_block) * kHalf + at * P.box_rows * 128, kv ? &VM : &KM, 64 * (n / per_block), in_page, p.h, page, smem_addr(bar));
-          }
-          if (cut) {
-            ok = t5_wait_warp(&tail_full, tails++ & 1, P.wait_limit, P.a.err, abort_flag);
-            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-            uint8_t* dst = smem_raw + (stage - smem_addr(smem_raw));
-            for (int n = lane; n < kPosBlock * halves * 8; n += 32) {
-              const int row = (n >> 3) & 127, half = n >> 10;
-              if (row >= end || row < begin) *reinterpret_cast<uint4*>(dst + half * kHalf + row * 128 + (n & 7) * 16) = zero;
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full + s);
-          }
-          if (++s == kStages) {
-            s = 0;
-            ph ^= 1u;
-          }
-        }
-      }
-    }
-    // copies still in flight land before the block gives its shared memory back
-    if (lane == 0) {
-      for (int i = 0; i < kStages; ++i) mbar_wait(smem_addr(full + i), i < s ? ph : ph ^ 1u, P.a.err, 1u << 16);
-      for (int x = 0; x < 2; ++x)
-        if (q_count[x]) mbar_wait(smem_addr(q_full + x), (q_count[x] & 1) ^ 1, P.a.err, 1u << 16);
-    }
-    __syncwarp();
-  } else if (warp == 1) {   // ----------------------------------------------------------- multiplications
-    if (lane == 0) {
-      constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
-      const uint32_t idesc_s = idesc_f16_m128(kPosBlock) | type, idesc_o = idesc_f16_m128(P.dim16) | type | (1u << 16);   // bit 16: V is position-major
-      const int steps = P.dim16 / 16;
-      int s = 0, q_count[2] = {0, 0}, p_count[2] = {0, 0};
-      uint32_t ph = 0;
-      bool ok = true;
-      auto take = [&](uint32_t& stage) -> bool {   // the next stage of the ring
-        if (!t5_wait(full + s, ph, P.wait_limit, P.a.err, abort_flag)) return false;
-        stage = s;
-        if (++s == kStages) {
-          s = 0;
-          ph ^= 1u;
-        }
-        return true;
-      };
-      auto scores = [&](int x, uint32_t stage, bool last) {
-        tc_fence_after();
-        const uint64_t q = smem_desc_sw128(base + x * Z::kTile), k = smem_desc_sw128(ring + stage * Z::kTile);
-        for (int i = 0; i < steps; ++i) {   // 32 bytes further inside the swizzle row; then the other half
-          const uint32_t off = (i & 3) * 2 + (i >> 2) * (kHalf >> 4);
-          mma_ss_f16(tmem + x * 128, q + off, k + off, idesc_s, i > 0);
-        }
-        mma_commit(s_full + x);
-        if (last) mma_commit(q_empty + x);
-      };
-      while (walk.left > 0 && ok) {
-        const Piece p = next_piece(P, shape, walk);
-        const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
-        int j = p.j0;
-        while (j < p.j1 && !r[0].has(j) && !r[1].has(j)) ++j;
-        uint32_t k_stage = 0, v_stage = 0;
-        bool more = j < p.j1;
-        if (more) {   // the first scores
-          if (!(ok = take(k_stage))) break;
-          for (int x = 0; x < 2 && ok; ++x)
-            if (r[x].has(j)) {
-              if (!(ok = t5_wait(q_full + x, q_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
-              scores(x, k_stage, j + 1 == r[x].last);
-            }
-          mma_commit(empty + k_stage);
-        }
-        for (; more && ok; ++j) {
-          more = j + 1 < p.j1 && (r[0].has(j + 1) || r[1].has(j + 1));
-          if (!(ok = take(v_stage)) || (more && !(ok = take(k_stage)))) break;
-          const uint64_t v = (smem_desc_sw128(ring + v_stage * Z::kTile) & ~(0x3FFFull << 16)) | (static_cast<uint64_t>(kHalf >> 4) << 16);
-          for (int x = 0; x < 2 && ok; ++x) {
-            if (r[x].has(j)) {
-              if (!(ok = t5_wait(p_full + x, p_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
-              tc_fence_after();
-              for (int i = 0; i < 8; ++i)   // 16 positions further: two groups of eight rows
-                mma_ts_f16(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, v + i * (2048 >> 4), idesc_o, j > r[x].first || i > 0);
-              if (j + 1 == r[x].last) mma_commit(o_full + x);
-            }
-            if (more && r[x].has(j + 1)) {
-              if (j + 1 == r[x].first && !(ok = t5_wait(q_full + x, q_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
-              scores(x, k_stage, j + 2 == r[x].last);
-            }
-          }
-          mma_commit(empty + v_stage);
-          if (more) mma_commit(empty + k_stage);
-        }
-      }
-      mma_commit(&mma_done);   // they read shared memory and write tensor memory, which the block is about to give back
-      mbar_wait(smem_addr(&mma_done), 0, P.a.err, 1u << 16);
-    }
-    __syncwarp();
-  } else if (warp >= 4) {   // -------------------------------------------------------------- softmax
+  if (warp >= 4) {   // -------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptRegsSoftmax));   // the sum is what the block was launched with
     const int x = (warp >> 2) - 1, row = (warp & 3) * 32 + lane, token = row / P.group, head = row - token * P.group;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + lanes + x * 128, to = tmem + lanes + 256 + x * 128;
@@ -434,24 +317,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (!idle) {
           tc_fence_after();
           uint32_t v[128];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) tmem_load32(ts + 32 * k, v + 32 * k);
-          tmem_wait_load();
-          if (flip) {
-#pragma unroll
-            for (int k = 0; k < 128; ++k) v[k] ^= 0x80000000u;
-          }
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           const int p0 = j * kPosBlock;
-          if (p0 + kPosBlock - 1 > r.p_first || (P.a.window > 0 && p0 <= r.p_last - P.a.window)) {   // some row does not see all of it
-            const int top = pos - p0, bottom = lo - p0;
+          const bool masked = p0 + kPosBlock - 1 > r.p_first || (P.a.window > 0 && p0 <= r.p_last - P.a.window);   // some row does not see all of it
+          tmem_load32(ts, v);
 #pragma unroll
-            for (int k = 0; k < 128; ++k)
-              if (k > top || k < bottom) v[k] = 0xff800000u;
+          for (int k = 0; k < 4; ++k) {   // a quarter is looked through while the next one comes
+            tmem_wait_load();
+            if (k < 3) tmem_load32(ts + 32 * (k + 1), v + 32 * (k + 1));
+            if (flip) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[32 * k + i] ^= 0x80000000u;
+            }
+            if (masked) {
+              const int top = pos - p0, bottom = lo - p0;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (32 * k + i > top || 32 * k + i < bottom) v[32 * k + i] = 0xff800000u;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(v[32 * k + i]), __uint_as_float(v[32 * k + i + 1]));
           }
-          float mx = -INFINITY;
-#pragma unroll
-          for (int k = 0; k < 128; ++k) mx = fmaxf(mx, __uint_as_float(v[k]));
-          mx *= c;
+          const float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * c;
           const bool grow = mx > m + kSlack;
           if (__any_sync(0xffffffffu, grow)) {
             const float m2 = grow ? mx : m, keep = m == -INFINITY ? 0.f : exp2_fast(m - m2);   // nothing seen yet: O and l count for nothing
@@ -470,24 +357,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
           }
           const float ref = m == -INFINITY ? 0.f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const float2 c2 = make_float2(c, c), ref2 = make_float2(-ref, -ref);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            uint32_t h[8];
+          for (int k = 0; k < 4; ++k) {
+            uint32_t h[16];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float e0 = exp2_fast(fmaf(__uint_as_float(v[16 * k + 2 * i]), c, -ref)), e1 = exp2_fast(fmaf(__uint_as_float(v[16 * k + 2 * i + 1]), c, -ref));
-              sum[(2 * i) & 3] += e0;
-              sum[(2 * i + 1) & 3] += e1;
-              h[i] = pack2<T>(e0, e1);
+            for (int i = 0; i < 16; ++i) {
+              const float2 e = fma2(make_float2(__uint_as_float(v[32 * k + 2 * i]), __uint_as_float(v[32 * k + 2 * i + 1])), c2, ref2);
+              const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+              sum[i & 1] = add2(sum[i & 1], w);
+              h[i] = pack2<T>(w.x, w.y);
             }
-            asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(ts + 8 * k), "r"(h[0]), "r"(h[1]), "r"(h[2]),
-                         "r"(h[3]), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7])
-                         : "memory");
+            tmem_store16(ts + 16 * k, h);
+            if (k == 1) {
+              tmem_wait_store();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(p_half + x);
+            }
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
           tmem_wait_store();
           tc_fence_before();
+        } else if (lane == 0) {
+          mbar_arrive(p_half + x);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + x);
@@ -533,6 +427,157 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       }
       tc_fence_before();   // the next P is announced after these reads of O
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptRegsOther));
+    if (warp == 0) {   // ---------------------------------------------------------------- loads
+      int s = 0, q_count[2] = {0, 0}, tails = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      const int per_block = kPosBlock / P.box_rows, halves = DP / 64, n_boxes = per_block * halves;
+      while (walk.left > 0 && ok) {
+        const Piece p = next_piece(P, shape, walk);
+        const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
+        for (int x = 0; x < 2 && ok; ++x) {
+          if (r[x].none()) continue;
+          if (!(ok = t5_wait_warp(q_empty + x, (q_count[x] & 1) ^ 1, P.wait_limit, P.a.err, abort_flag))) break;
+          ++q_count[x];
+          if (lane == 0) {
+            mbar_expect(q_full + x, halves * 128u * P.group * P.tile_tokens);
+            for (int d = 0; d < halves; ++d)
+              tma_load_3d(base + x * Z::kTile + d * kHalf, &QM, 64 * d, p.h * P.group, p.s.row0 + p.t0 + x * P.tile_tokens, smem_addr(q_full + x));
+          }
+        }
+        // positions that some row of the pair sees
+        const PairRange pr = pair_range(shape, p.s.q, p.t0 / shape.pair_tokens);
+        const int* table = P.a.seq.table + p.b * P.a.seq.table_stride;
+        for (int j = p.j0; j < p.j1 && ok; ++j) {
+          if (!r[0].has(j) && !r[1].has(j)) continue;
+          const int end = min(kPosBlock, pr.hi - j * kPosBlock), begin = max(0, pr.lo - j * kPosBlock);
+          const int rows_end = (end + P.box_rows - 1) / P.box_rows, rows_begin = begin / P.box_rows, count = (rows_end - rows_begin) * halves;
+          // lane n < n_boxes: box n % per_block of half n / per_block
+          int page = 0, in_page = 0;
+          const int at = lane % per_block;
+          const bool mine = lane < n_boxes && at >= rows_begin && at < rows_end;
+          if (mine) {
+            const int pos = j * kPosBlock + at * P.box_rows, column = pos / P.a.pool.page_size;
+            page = table[column];
+            in_page = pos - column * P.a.pool.page_size;
+            if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(P.a.pool.n_pages)) {   // the tensor map's bounds fill it with zeros
+              atomicOr(P.a.err, kErrWordIndex);
+              page = P.a.pool.n_pages;
+            }
+          }
+          for (int kv = 0; kv < 2 && ok; ++kv) {
+            if (!(ok = t5_wait_warp(empty + s, ph ^ 1u, P.wait_limit, P.a.err, abort_flag))) break;
+            const uint32_t stage = ring + s * Z::kTile;
+            const bool cut = kv == 1 && (end < kPosBlock || begin > 0);
+            uint64_t* bar = cut ? &tail_full : full + s;
+            if (lane == 0) mbar_expect(bar, count * P.box_rows * 128u);
+            __syncwarp();
+            for (int n = lane; n < n_boxes; n += 32) {   // at most 32 boxes: box_rows is at least 8, halves at most 2
+              if (mine) tma_load_4d(stage + (n / per_block) * kHalf + at * P.box_rows * 128, kv ? &VM : &KM, 64 * (n / per_block), in_page, p.h, page, smem_addr(bar));
+            }
+            if (cut) {
+              ok = t5_wait_warp(&tail_full, tails++ & 1, P.wait_limit, P.a.err, abort_flag);
+              const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+              uint8_t* dst = smem_raw + (stage - smem_addr(smem_raw));
+              for (int n = lane; n < kPosBlock * halves * 8; n += 32) {
+                const int row = (n >> 3) & 127, half = n >> 10;
+                if (row >= end || row < begin) *reinterpret_cast<uint4*>(dst + half * kHalf + row * 128 + (n & 7) * 16) = zero;
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) mbar_arrive(full + s);
+            }
+            if (++s == kStages) {
+              s = 0;
+              ph ^= 1u;
+            }
+          }
+        }
+      }
+      // copies still in flight land before the block gives its shared memory back
+      if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) mbar_wait(smem_addr(full + i), i < s ? ph : ph ^ 1u, P.a.err, 1u << 16);
+        for (int x = 0; x < 2; ++x)
+          if (q_count[x]) mbar_wait(smem_addr(q_full + x), (q_count[x] & 1) ^ 1, P.a.err, 1u << 16);
+      }
+      __syncwarp();
+    } else if (warp == 1) {   // ----------------------------------------------------------- multiplications
+      if (lane == 0) {
+        constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
+        const uint32_t idesc_s = idesc_f16_m128(kPosBlock) | type, idesc_o = idesc_f16_m128(P.dim16) | type | (1u << 16);   // bit 16: V is position-major
+        const int steps = P.dim16 / 16;
+        int s = 0, q_count[2] = {0, 0}, p_count[2] = {0, 0};
+        uint32_t ph = 0;
+        bool ok = true;
+        auto take = [&](uint32_t& stage) -> bool {   // the next stage of the ring
+          if (!t5_wait(full + s, ph, P.wait_limit, P.a.err, abort_flag)) return false;
+          stage = s;
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1u;
+          }
+          return true;
+        };
+        auto scores = [&](int x, uint32_t stage, bool last) {
+          tc_fence_after();
+          const uint64_t q = smem_desc_sw128(base + x * Z::kTile), k = smem_desc_sw128(ring + stage * Z::kTile);
+          for (int i = 0; i < steps; ++i) {   // 32 bytes further inside the swizzle row; then the other half
+            const uint32_t off = (i & 3) * 2 + (i >> 2) * (kHalf >> 4);
+            mma_ss_f16(tmem + x * 128, q + off, k + off, idesc_s, i > 0);
+          }
+          mma_commit(s_full + x);
+          if (last) mma_commit(q_empty + x);
+        };
+        while (walk.left > 0 && ok) {
+          const Piece p = next_piece(P, shape, walk);
+          const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
+          int j = p.j0;
+          while (j < p.j1 && !r[0].has(j) && !r[1].has(j)) ++j;
+          uint32_t k_stage = 0, v_stage = 0;
+          bool more = j < p.j1;
+          if (more) {   // the first scores
+            if (!(ok = take(k_stage))) break;
+            for (int x = 0; x < 2 && ok; ++x)
+              if (r[x].has(j)) {
+                if (!(ok = t5_wait(q_full + x, q_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+                scores(x, k_stage, j + 1 == r[x].last);
+              }
+            mma_commit(empty + k_stage);
+          }
+          for (; more && ok; ++j) {
+            more = j + 1 < p.j1 && (r[0].has(j + 1) || r[1].has(j + 1));
+            if (!(ok = take(v_stage)) || (more && !(ok = take(k_stage)))) break;
+            const uint64_t v = (smem_desc_sw128(ring + v_stage * Z::kTile) & ~(0x3FFFull << 16)) | (static_cast<uint64_t>(kHalf >> 4) << 16);
+            for (int x = 0; x < 2 && ok; ++x) {
+              if (r[x].has(j)) {
+                if (!(ok = t5_wait(p_half + x, p_count[x] & 1, P.wait_limit, P.a.err, abort_flag))) break;
+                tc_fence_after();
+  #pragma unroll
+                for (int i = 0; i < 4; ++i)   // 16 positions further: two groups of eight rows
+                  mma_ts_f16(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, v + i * (2048 >> 4), idesc_o, j > r[x].first || i > 0);
+                if (!(ok = t5_wait(p_full + x, p_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+                tc_fence_after();
+  #pragma unroll
+                for (int i = 4; i < 8; ++i)
+                  mma_ts_f16(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, v + i * (2048 >> 4), idesc_o, true);
+                if (j + 1 == r[x].last) mma_commit(o_full + x);
+              }
+              if (more && r[x].has(j + 1)) {
+                if (j + 1 == r[x].first && !(ok = t5_wait(q_full + x, q_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+                scores(x, k_stage, j + 2 == r[x].last);
+              }
+            }
+            mma_commit(empty + v_stage);
+            if (more) mma_commit(empty + k_stage);
+          }
+        }
+        mma_commit(&mma_done);   // they read shared memory and write tensor memory, which the block is about to give back
+        mbar_wait(smem_addr(&mma_done), 0, P.a.err, 1u << 16);
+      }
+      __syncwarp();
     }
   }
   tc_fence_before();
