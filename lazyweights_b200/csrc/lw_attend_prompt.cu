@@ -49,6 +49,7 @@ struct PromptArgs {
   int dim16;                // head_dim rounded up to 16
   int cap;                  // positions the table can name
   uint32_t wait_limit;
+  int drop;                 // a test's lost copy: block 0 never loads this block of keys of its share (-1: none)
   PieceNote* notes;         // [gridDim.x]
   float* partial;           // [gridDim.x][piece][tile]: m[128], l[128], O [dim16 / 4][128][4]
 };
@@ -430,22 +431,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptRegsOther));
-    if (warp == 0) {   // ---------------------------------------------------------------- loads
-      int s = 0, q_count[2] = {0, 0}, tails = 0;
+    if (warp == 0 || warp == 2) {   // ------------------------------------------------------- loads: warp 0 queries and keys, warp 2 values
+      const bool values = warp == 2;
+      const void* const map = values ? &VM : &KM;
+      int s = values, q_count[2] = {0, 0}, tails = 0, fills = 0;
       uint32_t ph = 0;
       bool ok = true;
-      const int per_block = kPosBlock / P.box_rows, halves = DP / 64, n_boxes = per_block * halves;
+      constexpr int kHalves = DP / 64;
+      const int per_block = kPosBlock / P.box_rows;   // at most 16
       while (walk.left > 0 && ok) {
         const Piece p = next_piece(P, shape, walk);
         const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
-        for (int x = 0; x < 2 && ok; ++x) {
-          if (r[x].none()) continue;
-          if (!(ok = t5_wait_warp(q_empty + x, (q_count[x] & 1) ^ 1, P.wait_limit, P.a.err, abort_flag))) break;
-          ++q_count[x];
-          if (lane == 0) {
-            mbar_expect(q_full + x, halves * 128u * P.group * P.tile_tokens);
-            for (int d = 0; d < halves; ++d)
-              tma_load_3d(base + x * Z::kTile + d * kHalf, &QM, 64 * d, p.h * P.group, p.s.row0 + p.t0 + x * P.tile_tokens, smem_addr(q_full + x));
+        if (!values) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (r[x].none() || !ok) continue;
+            if (!(ok = t5_wait_warp(q_empty + x, (q_count[x] & 1) ^ 1, P.wait_limit, P.a.err, abort_flag))) continue;
+            ++q_count[x];
+            if (elect_one()) {
+              mbar_expect(q_full + x, kHalves * 128u * P.group * P.tile_tokens);
+#pragma unroll
+              for (int d = 0; d < kHalves; ++d)
+                tma_load_3d(base + x * Z::kTile + d * kHalf, &QM, 64 * d, p.h * P.group, p.s.row0 + p.t0 + x * P.tile_tokens, smem_addr(q_full + x));
+            }
+            __syncwarp();
           }
         }
         // positions that some row of the pair sees
@@ -454,13 +463,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int j = p.j0; j < p.j1 && ok; ++j) {
           if (!r[0].has(j) && !r[1].has(j)) continue;
           const int end = min(kPosBlock, pr.hi - j * kPosBlock), begin = max(0, pr.lo - j * kPosBlock);
-          const int rows_end = (end + P.box_rows - 1) / P.box_rows, rows_begin = begin / P.box_rows, count = (rows_end - rows_begin) * halves;
-          // lane n < n_boxes: box n % per_block of half n / per_block
+          const int rows_end = (end + P.box_rows - 1) / P.box_rows, rows_begin = begin / P.box_rows;
+          // lane n: the page of box n
           int page = 0, in_page = 0;
-          const int at = lane % per_block;
-          const bool mine = lane < n_boxes && at >= rows_begin && at < rows_end;
-          if (mine) {
-            const int pos = j * kPosBlock + at * P.box_rows, column = pos / P.a.pool.page_size;
+          if (lane >= rows_begin && lane < rows_end) {
+            const int pos = j * kPosBlock + lane * P.box_rows, column = pos / P.a.pool.page_size;
             page = table[column];
             in_page = pos - column * P.a.pool.page_size;
             if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(P.a.pool.n_pages)) {   // the tensor map's bounds fill it with zeros
@@ -468,115 +475,126 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               page = P.a.pool.n_pages;
             }
           }
-          for (int kv = 0; kv < 2 && ok; ++kv) {
-            if (!(ok = t5_wait_warp(empty + s, ph ^ 1u, P.wait_limit, P.a.err, abort_flag))) break;
-            const uint32_t stage = ring + s * Z::kTile;
-            const bool cut = kv == 1 && (end < kPosBlock || begin > 0);
-            uint64_t* bar = cut ? &tail_full : full + s;
-            if (lane == 0) mbar_expect(bar, count * P.box_rows * 128u);
+          if (!(ok = t5_wait_warp(empty + s, ph ^ 1u, P.wait_limit, P.a.err, abort_flag))) break;
+          const uint32_t stage = ring + s * Z::kTile;
+          const bool cut = values && (end < kPosBlock || begin > 0);
+          uint64_t* const bar = cut ? &tail_full : full + s;
+          if (fills++ != P.drop || values || blockIdx.x != 0) {
+            if (elect_one()) mbar_expect(bar, (rows_end - rows_begin) * kHalves * P.box_rows * 128u);
             __syncwarp();
-            for (int n = lane; n < n_boxes; n += 32) {   // at most 32 boxes: box_rows is at least 8, halves at most 2
-              if (mine) tma_load_4d(stage + (n / per_block) * kHalf + at * P.box_rows * 128, kv ? &VM : &KM, 64 * (n / per_block), in_page, p.h, page, smem_addr(bar));
-            }
-            if (cut) {
-              ok = t5_wait_warp(&tail_full, tails++ & 1, P.wait_limit, P.a.err, abort_flag);
-              const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-              uint8_t* dst = smem_raw + (stage - smem_addr(smem_raw));
-              for (int n = lane; n < kPosBlock * halves * 8; n += 32) {
-                const int row = (n >> 3) & 127, half = n >> 10;
-                if (row >= end || row < begin) *reinterpret_cast<uint4*>(dst + half * kHalf + row * 128 + (n & 7) * 16) = zero;
+            for (int n = rows_begin; n < rows_end; ++n) {
+              const int pg = __shfl_sync(0xffffffffu, page, n), in = __shfl_sync(0xffffffffu, in_page, n);
+              if (elect_one()) {
+#pragma unroll
+                for (int d = 0; d < kHalves; ++d) tma_load_4d(stage + d * kHalf + n * P.box_rows * 128, map, 64 * d, in, p.h, pg, smem_addr(bar));
               }
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
               __syncwarp();
-              if (lane == 0) mbar_arrive(full + s);
             }
-            if (++s == kStages) {
-              s = 0;
-              ph ^= 1u;
+          }
+          if (cut) {
+            ok = t5_wait_warp(&tail_full, tails++ & 1, P.wait_limit, P.a.err, abort_flag);
+            uint8_t* dst = smem_raw + (stage - smem_addr(smem_raw));
+            for (int n = lane; n < kPosBlock * kHalves * 8; n += 32) {
+              const int row = (n >> 3) & 127, half = n >> 10;
+              if (row >= end || row < begin) *reinterpret_cast<uint4*>(dst + half * kHalf + row * 128 + (n & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (elect_one()) mbar_arrive(full + s);
+            __syncwarp();
+          }
+          s += 2;   // the ring holds keys and values in turn
+          if (s >= kStages) {
+            s -= kStages;
+            ph ^= 1u;
           }
         }
       }
-      // copies still in flight land before the block gives its shared memory back
-      if (lane == 0) {
-        for (int i = 0; i < kStages; ++i) mbar_wait(smem_addr(full + i), i < s ? ph : ph ^ 1u, P.a.err, 1u << 16);
-        for (int x = 0; x < 2; ++x)
-          if (q_count[x]) mbar_wait(smem_addr(q_full + x), (q_count[x] & 1) ^ 1, P.a.err, 1u << 16);
-      }
-      __syncwarp();
-    } else if (warp == 1) {   // ----------------------------------------------------------- multiplications
-      if (lane == 0) {
-        constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
-        const uint32_t idesc_s = idesc_f16_m128(kPosBlock) | type, idesc_o = idesc_f16_m128(P.dim16) | type | (1u << 16);   // bit 16: V is position-major
-        const int steps = P.dim16 / 16;
-        int s = 0, q_count[2] = {0, 0}, p_count[2] = {0, 0};
-        uint32_t ph = 0;
-        bool ok = true;
-        auto take = [&](uint32_t& stage) -> bool {   // the next stage of the ring
-          if (!t5_wait(full + s, ph, P.wait_limit, P.a.err, abort_flag)) return false;
-          stage = s;
-          if (++s == kStages) {
-            s = 0;
-            ph ^= 1u;
-          }
-          return true;
-        };
-        auto scores = [&](int x, uint32_t stage, bool last) {
-          tc_fence_after();
-          const uint64_t q = smem_desc_sw128(base + x * Z::kTile), k = smem_desc_sw128(ring + stage * Z::kTile);
-          for (int i = 0; i < steps; ++i) {   // 32 bytes further inside the swizzle row; then the other half
+    } else if (warp == 1) {   // ----------------------------------------------------------- multiplications, started by one lane
+      constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
+      const uint32_t idesc_s = idesc_f16_m128(kPosBlock) | type, idesc_o = idesc_f16_m128(P.dim16) | type | (1u << 16);   // bit 16: V is position-major
+      const int steps = P.dim16 / 16;
+      int s = 0, q_count[2] = {0, 0}, p_count[2] = {0, 0};
+      uint32_t ph = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int parity) -> bool {
+        if (ok) ok = t5_wait_warp(bar, parity, P.wait_limit, P.a.err, abort_flag);
+        tc_fence_after();
+        return ok;
+      };
+      auto take = [&](uint32_t& stage) -> bool {   // the next stage of the ring
+        stage = s;
+        wait(full + s, ph);
+        if (++s == kStages) {
+          s = 0;
+          ph ^= 1u;
+        }
+        return ok;
+      };
+      auto scores = [&](int x, uint32_t stage, bool last) {
+        const uint64_t q = smem_desc_sw128(base + x * Z::kTile), k = smem_desc_sw128(ring + stage * Z::kTile);
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < DP / 16; ++i) {   // 32 bytes further inside the swizzle row; then the other half
             const uint32_t off = (i & 3) * 2 + (i >> 2) * (kHalf >> 4);
-            mma_ss_f16(tmem + x * 128, q + off, k + off, idesc_s, i > 0);
+            if (i < steps) mma_ss_f16(tmem + x * 128, q + off, k + off, idesc_s, i > 0);
           }
           mma_commit(s_full + x);
           if (last) mma_commit(q_empty + x);
-        };
-        while (walk.left > 0 && ok) {
-          const Piece p = next_piece(P, shape, walk);
-          const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
-          int j = p.j0;
-          while (j < p.j1 && !r[0].has(j) && !r[1].has(j)) ++j;
-          uint32_t k_stage = 0, v_stage = 0;
-          bool more = j < p.j1;
-          if (more) {   // the first scores
-            if (!(ok = take(k_stage))) break;
-            for (int x = 0; x < 2 && ok; ++x)
-              if (r[x].has(j)) {
-                if (!(ok = t5_wait(q_full + x, q_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
-                scores(x, k_stage, j + 1 == r[x].last);
-              }
-            mma_commit(empty + k_stage);
-          }
-          for (; more && ok; ++j) {
-            more = j + 1 < p.j1 && (r[0].has(j + 1) || r[1].has(j + 1));
-            if (!(ok = take(v_stage)) || (more && !(ok = take(k_stage)))) break;
-            const uint64_t v = (smem_desc_sw128(ring + v_stage * Z::kTile) & ~(0x3FFFull << 16)) | (static_cast<uint64_t>(kHalf >> 4) << 16);
-            for (int x = 0; x < 2 && ok; ++x) {
-              if (r[x].has(j)) {
-                if (!(ok = t5_wait(p_half + x, p_count[x] & 1, P.wait_limit, P.a.err, abort_flag))) break;
-                tc_fence_after();
-  #pragma unroll
+        }
+        __syncwarp();
+      };
+      while (walk.left > 0 && ok) {
+        const Piece p = next_piece(P, shape, walk);
+        const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
+        int j = p.j0;
+        while (j < p.j1 && !r[0].has(j) && !r[1].has(j)) ++j;
+        uint32_t k_stage = 0, v_stage = 0;
+        bool more = j < p.j1;
+        if (more) {   // the first scores
+          if (!take(k_stage)) break;
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            if (r[x].has(j) && wait(q_full + x, q_count[x]++ & 1)) scores(x, k_stage, j + 1 == r[x].last);
+          if (elect_one()) mma_commit(empty + k_stage);
+          __syncwarp();
+        }
+        for (; more && ok; ++j) {
+          more = j + 1 < p.j1 && (r[0].has(j + 1) || r[1].has(j + 1));
+          if (!take(v_stage) || (more && !take(k_stage))) break;
+          const uint64_t v = (smem_desc_sw128(ring + v_stage * Z::kTile) & ~(0x3FFFull << 16)) | (static_cast<uint64_t>(kHalf >> 4) << 16);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (r[x].has(j) && wait(p_half + x, p_count[x] & 1)) {
+              const bool fresh = j == r[x].first, last = j + 1 == r[x].last;
+              if (elect_one()) {
+#pragma unroll
                 for (int i = 0; i < 4; ++i)   // 16 positions further: two groups of eight rows
-                  mma_ts_f16(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, v + i * (2048 >> 4), idesc_o, j > r[x].first || i > 0);
-                if (!(ok = t5_wait(p_full + x, p_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
-                tc_fence_after();
-  #pragma unroll
-                for (int i = 4; i < 8; ++i)
-                  mma_ts_f16(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, v + i * (2048 >> 4), idesc_o, true);
-                if (j + 1 == r[x].last) mma_commit(o_full + x);
+                  mma_ts_f16(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, v + i * (2048 >> 4), idesc_o, !fresh || i > 0);
               }
-              if (more && r[x].has(j + 1)) {
-                if (j + 1 == r[x].first && !(ok = t5_wait(q_full + x, q_count[x]++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
-                scores(x, k_stage, j + 2 == r[x].last);
+              __syncwarp();
+              if (wait(p_full + x, p_count[x]++ & 1)) {
+                if (elect_one()) {
+#pragma unroll
+                  for (int i = 4; i < 8; ++i)
+                    mma_ts_f16(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, v + i * (2048 >> 4), idesc_o, true);
+                  if (last) mma_commit(o_full + x);
+                }
+                __syncwarp();
               }
             }
+            if (more && r[x].has(j + 1) && (j + 1 > r[x].first || wait(q_full + x, q_count[x]++ & 1)) && ok) scores(x, k_stage, j + 2 == r[x].last);
+          }
+          if (elect_one()) {
             mma_commit(empty + v_stage);
             if (more) mma_commit(empty + k_stage);
           }
+          __syncwarp();
         }
-        mma_commit(&mma_done);   // they read shared memory and write tensor memory, which the block is about to give back
-        mbar_wait(smem_addr(&mma_done), 0, P.a.err, 1u << 16);
       }
+      if (elect_one()) mma_commit(&mma_done);   // they read shared memory and write tensor memory, which the block is about to give back
+      __syncwarp();
+      if (lane == 0) mbar_wait(smem_addr(&mma_done), 0, P.a.err, 1u << 16);
       __syncwarp();
     }
   }
@@ -585,6 +603,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+  // Every copy has been waited for by the multiplications, unless the block gave up: then those in flight land before it gives its
+  // shared memory back (both parities: one of them has passed).
+  if (abort_word && warp == 0 && lane == 0) {
+    for (int i = 0; i < kStages; ++i)
+      for (int parity = 0; parity < 2; ++parity) mbar_wait(smem_addr(full + i), parity, P.a.err, 1u << 14);
+    for (int x = 0; x < 2; ++x)
+      for (int parity = 0; parity < 2; ++parity) mbar_wait(smem_addr(q_full + x), parity, P.a.err, 1u << 14);
   }
 }
 
@@ -675,6 +701,7 @@ int launch_attend_prompt(const PagedCache& cache, const AttendArgs& a, cudaStrea
   p.dim16 = (a.pool.Dh + 15) / 16 * 16;
   p.cap = static_cast<int>(std::min<long long>(static_cast<long long>(a.seq.table_cols) * a.pool.page_size, 1 << 30));
   p.wait_limit = debug_knobs().wait_limit;
+  p.drop = debug_knobs().drop_unit;
   p.notes = static_cast<PieceNote*>(a.workspace);
   p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + notes_bytes(sm_count()));
   alignas(64) CUtensorMap qm, km, vm;

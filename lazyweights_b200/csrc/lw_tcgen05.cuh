@@ -91,6 +91,14 @@ __host__ __device__ constexpr uint32_t idesc_f16_m128(int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
 }
 
+// True in one lane of a converged warp, the same one every time.  What a lane chosen this way issues is known to come from
+// a single thread, so its operands may stay in uniform registers: with `lane == 0` instead, an MMA took 78 cycles to issue.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 // bounded waits that also end when another warp of the block has given up
 __device__ __forceinline__ bool t5_wait(uint64_t* bar, uint32_t parity, uint32_t limit, unsigned int* err, volatile int* abort_flag) {
   const uint32_t addr = smem_addr(bar);
