@@ -2,9 +2,10 @@
 // arithmetic for host and device.
 //
 // Prompts: the query rows of one kv head are (token, head of its group), token by token; a tile of 128 rows holds
-// 128 / group tokens, a pair of tiles `pair_tokens` = twice that.  The work of a pair is one unit per block of 128 positions
-// that any of its tokens sees, one at least.  Units are numbered sequence by sequence, kv head by kv head, pair by pair,
-// position block by position block; block c of G takes the units c U / G .. (c + 1) U / G - 1 of U.
+// 128 / group tokens, a pair of tiles `pair_tokens` = twice that.  The work of a pair is `lead` units for what it costs besides
+// (queries in, results out, the pipeline's start), then one unit per block of 128 positions that any of its tokens sees, one at
+// least.  Units are numbered sequence by sequence, kv head by kv head, pair by pair, position block by position block; block c of
+// G takes the units c U / G .. (c + 1) U / G - 1 of U.
 #pragma once
 #include <cstdint>
 
@@ -42,7 +43,7 @@ LW_HD long long floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
 }
 
 struct PromptShape {
-  int pair_tokens, window;
+  int pair_tokens, window, lead;
 };
 
 // One sequence: `rows` new tokens, the last of its `len` positions.
@@ -72,10 +73,10 @@ LW_HD long long units_before(const PromptShape& s, const PromptSeq& q, int i) {
   if (i <= 0) return 0;
   const int pairs = prompt_pairs(s, q), T = s.pair_tokens, p0 = q.len - q.rows;
   const int whole = i < pairs ? i : pairs - 1;   // pairs of T tokens each: hi = p0 + (k + 1) T
-  long long sum = 0;
+  long long sum = static_cast<long long>(i) * s.lead;
   if (i == pairs) {
     const PairRange r = pair_range(s, q, pairs - 1);
-    sum = r.last - r.first;
+    sum += r.last - r.first;
   }
   // pairs that end at or before position 0: one unit each
   int none = 0;

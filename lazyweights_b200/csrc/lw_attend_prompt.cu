@@ -31,9 +31,10 @@
 
 namespace lw {
 
-constexpr int kPromptThreads = 12 * 32;
-constexpr int kPromptRegsSoftmax = 208, kPromptRegsOther = 88;   // 8 and 4 warps: 12 x 168, the launch's
+constexpr int kPromptThreads = 20 * 32;
 constexpr float kSlack = 8.f;
+constexpr int kPolyEvery = 4;
+constexpr int kPromptLead = 2;
 
 // The pair that block c continues: its first packed row, rows (tokens) and first query head, and the blocks that hold its first and
 // last unit (first == c: none).  A block leaves the pair that it continues as its piece 0, the one that it only begins as piece 1.
@@ -81,15 +82,16 @@ struct Piece {
   SeqRows s;
   int b;
 };
+// A piece without position blocks (j0 == j1) is to be passed over.
 __device__ __forceinline__ Piece next_piece(const PromptArgs& P, const PromptShape& shape, Walk& w) {
   const PairRange r = pair_range(shape, w.s.q, w.i);
-  const int n = r.last - r.first, take = static_cast<int>(min(static_cast<long long>(n - w.off), w.left));
+  const int n = shape.lead + r.last - r.first, take = static_cast<int>(min(static_cast<long long>(n - w.off), w.left));
   Piece p;
   p.h = w.h;
   p.t0 = w.i * shape.pair_tokens;
-  p.j0 = r.first + w.off;
-  p.j1 = p.j0 + take;
-  p.begins = w.off == 0;
+  p.j0 = r.first + max(0, w.off - shape.lead);
+  p.j1 = r.first + max(0, w.off + take - shape.lead);
+  p.begins = w.off <= shape.lead;
   p.ends = w.off + take == n;
   p.s = w.s;
   p.b = w.b;
@@ -143,6 +145,26 @@ __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* v) {
       : "memory");
 }
 
+// t5_wait for a converged warp whose lanes leave the loop together: 60 cycles where the barrier is ready; with a way out per lane 160.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, uint32_t limit, unsigned int* err, volatile int* abort_flag) {
+  const uint32_t addr = smem_addr(bar);
+  for (uint32_t i = 0; i < limit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, done != 0)) return true;
+    if ((i & 63u) == 63u && __any_sync(0xffffffffu, *abort_flag != 0)) return false;
+  }
+  atomicOr(err, 1u);
+  *abort_flag = 1;
+  return false;
+}
+
 // Two 32-bit operations in one instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
@@ -158,6 +180,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
+// 2^x without the special-function unit, which gives 16 results per cycle and SM where the rest of the softmax could take twice
+// that: x = n + f, n the nearest integer (the rounding of a sum with 1.5 x 2^23), 2^f by a cubic of least relative error over
+// |f| <= 1/2 (7.5e-5, a sixth of half a step of fp16; fitted by reweighted least squares), n added to the exponent.  Below 2^-126:
+// about 2^-126.  A NaN does not come through: a row with one has it in its reference, and the other half of its exponentials.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 shift = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f), minus = make_float2(-1.f, -1.f);
+  const float2 t = add2(x, shift), n = add2(t, back), f = fma2(n, minus, x);
+  float2 p = fma2(f, make_float2(0.05517167f, 0.05517167f), make_float2(0.24261113f, 0.24261113f));
+  p = fma2(p, f, make_float2(0.69326099f, 0.69326099f));
+  p = fma2(p, f, make_float2(0.99992807f, 0.99992807f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
 // The largest of three; a NaN stays
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -169,7 +205,7 @@ template <int DP>
 struct PromptSizes {
   static constexpr uint32_t kTile = 128 * DP * 2;                   // bytes of a tile of queries, a block of keys or of values
   static constexpr int kStages = DP == 128 ? 5 : 8;
-  static constexpr size_t kSmem = 1024 + 2 * kTile + kStages * kTile;
+  static constexpr size_t kSmem = (2 + kStages) * kTile;   // and 3 KB of static variables: all that a block can have
 };
 
 template <typename T, int DP>
@@ -180,28 +216,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   constexpr int kStages = Z::kStages;
   constexpr uint32_t kHalf = 128 * 128;   // bytes of 64 columns of a tile: 128 rows of 128 bytes, swizzled
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], tail_full, mma_done;
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], mma_done[2], tail_full;
   __shared__ uint32_t tmem_slot[1];
   __shared__ int abort_word, s_first[4];
-  __shared__ long long s_scan[kPromptThreads / 32 + 1], s_rest;
+  __shared__ long long s_scan[kPromptThreads / 32], s_rest;
+  __shared__ float s_max[2][2][128];   // what the two threads of a row tell each other: [tile][half of the block][row]
   volatile int* abort_flag = &abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u, ring = base + 2 * Z::kTile;
+  const uint32_t base = smem_addr(smem_raw), ring = base + 2 * Z::kTile;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_addr(full + i), 1);
-      mbar_init(smem_addr(empty + i), 1);
+      mbar_init(smem_addr(empty + i), 2);   // both tiles
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(smem_addr(q_full + x), 1);
       mbar_init(smem_addr(q_empty + x), 1);
       mbar_init(smem_addr(s_full + x), 1);
-      mbar_init(smem_addr(p_half + x), 4);
-      mbar_init(smem_addr(p_full + x), 4);
+      mbar_init(smem_addr(p_full + x), 8);
       mbar_init(smem_addr(o_full + x), 1);
+      mbar_init(smem_addr(mma_done + x), 1);
     }
     mbar_init(smem_addr(&tail_full), 1);
-    mbar_init(smem_addr(&mma_done), 1);
     abort_word = 0;
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
@@ -213,7 +249,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   pdl_wait();
 
   // ---- this block's share of the units
-  const PromptShape shape = {2 * P.tile_tokens, P.a.window};
+  const PromptShape shape = {2 * P.tile_tokens, P.a.window, kPromptLead};
   const int n_seqs = P.a.seq.n;
   auto seq_units = [&](int b) -> long long {
     if (b >= n_seqs) return 0;
@@ -287,67 +323,100 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     walk.s = seq_rows(P, walk.b);
     if (tid == 0) {
       const PairRange r = pair_range(shape, walk.s.q, walk.i);
-      const long long begin = u0 - walk.off;   // unit u is block floor(((u + 1) blocks - 1) / units)'s
+      const long long begin = u0 - walk.off + shape.lead;   // of its position blocks; unit u is block floor(((u + 1) blocks - 1) / units)'s
       const int t0 = walk.i * shape.pair_tokens, me = blockIdx.x;
       P.notes[me] = {walk.s.row0 + t0, min(shape.pair_tokens, walk.s.q.rows - t0), walk.h * P.group,
-                     walk.off ? static_cast<int>(((begin + 1) * blocks - 1) / units) : me,
-                     walk.off ? static_cast<int>(((begin + r.last - r.first) * blocks - 1) / units) : me, {0, 0, 0}};
+                     walk.off > shape.lead ? static_cast<int>(((begin + 1) * blocks - 1) / units) : me,
+                     walk.off > shape.lead ? static_cast<int>(((begin + r.last - r.first) * blocks - 1) / units) : me, {0, 0, 0}};
     }
   }
 
   if (warp >= 4) {   // -------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptRegsSoftmax));   // the sum is what the block was launched with
-    const int x = (warp >> 2) - 1, row = (warp & 3) * 32 + lane, token = row / P.group, head = row - token * P.group;
+    // Two threads of a row, in two warps: 64 positions of a block each, and half of the row of O.
+    const int x = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, row = (warp & 3) * 32 + lane, token = row / P.group, head = row - token * P.group;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t ts = tmem + lanes + x * 128, to = tmem + lanes + 256 + x * 128;
-    const bool flip = P.a.scale < 0.f;
+    const uint32_t ts = tmem + lanes + x * 128 + 64 * half, to = tmem + lanes + 256 + x * 128;
+    const int pair_barrier = 1 + x * 4 + (warp & 3);
+    const int o_begin = half ? (P.dim16 / 32) * 16 : 0, o_end = half ? P.dim16 : (P.dim16 / 32) * 16;   // columns of O
     // a scale of 0 becomes a very small one: a score hidden as -inf must stay -inf
     const float c = fmaxf(fabsf(P.a.scale) * 1.4426950408889634f, 1e-30f);
-    int s_count = 0, o_count = 0;
+    const bool leading = half == 0 && (warp & 3) == 0, leader = leading && lane == 0;
+    int s_count = 0, o_count = 0, stage = 0, v_before = 0;
+    uint32_t stage_ph = 0;
     bool ok = true;
     while (walk.left > 0 && ok) {
       const Piece p = next_piece(P, shape, walk);
-      const TileRange r = tile_range(P, p, x);
+      if (p.j0 == p.j1) continue;
+      const TileRange r = tile_range(P, p, x), r2 = tile_range(P, p, x ^ 1);
       const bool mine = token < min(r.tokens, P.tile_tokens);
       const int pos = mine ? r.p_first + token : -1;
       const int lo = P.a.window > 0 ? max(0, pos - P.a.window + 1) : 0;
       const bool idle = !__any_sync(0xffffffffu, mine);
       float m = -INFINITY, l = 0.f;
-      for (int j = r.first; j < r.last; ++j) {
-        if (!(ok = t5_wait_warp(s_full + x, s_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+      for (int j = p.j0; j < p.j1; ++j) {
+        const bool here = r.has(j);
+        if (!here && !r2.has(j)) continue;
+        // The scores' completion tells that the multiplications are done with the keys of this block and the values of the one
+        // before: one thread per tile gives the stages back.  (A commit of its own for each would hold the tensor core up by 78 cycles.)
+        const int k_stage = stage, v_stage = k_stage + 1 == kStages ? 0 : k_stage + 1;
+        const uint32_t k_ph = stage_ph, v_ph = k_ph ^ (v_stage == 0 ? 1u : 0u);
+        stage = v_stage + 1 == kStages ? 0 : v_stage + 1;
+        stage_ph = v_ph ^ (stage == 0 ? 1u : 0u);
+        if (!here) {   // the other tile's: given back once it is there, so that the turns of a stage stay apart
+          if (leading) {
+            if (!(ok = wait_warp(full + k_stage, k_ph, P.wait_limit, P.a.err, abort_flag) && wait_warp(full + v_stage, v_ph, P.wait_limit, P.a.err, abort_flag))) break;
+            if (leader) {
+              mbar_arrive(empty + k_stage);
+              mbar_arrive(empty + v_stage);
+            }
+          }
+          continue;
+        }
+        if (!(ok = wait_warp(s_full + x, s_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+        if (leader) {
+          mbar_arrive(empty + k_stage);
+          if (j > r.first) mbar_arrive(empty + v_before);
+          if (j + 1 == r.last) mbar_arrive(q_empty + x);
+        }
+        v_before = v_stage;
         if (!idle) {
           tc_fence_after();
-          uint32_t v[128];
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          const int p0 = j * kPosBlock;
+          const int p0 = j * kPosBlock, top = pos - p0 - 64 * half, bottom = lo - p0 - 64 * half;
           const bool masked = p0 + kPosBlock - 1 > r.p_first || (P.a.window > 0 && p0 <= r.p_last - P.a.window);   // some row does not see all of it
-          tmem_load32(ts, v);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {   // a quarter is looked through while the next one comes
-            tmem_wait_load();
-            if (k < 3) tmem_load32(ts + 32 * (k + 1), v + 32 * (k + 1));
-            if (flip) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[32 * k + i] ^= 0x80000000u;
-            }
-            if (masked) {
-              const int top = pos - p0, bottom = lo - p0;
+          // S is read twice, for its maximum and for P: the code stays a few KB, which the instruction caches hold beside that of
+          // the warp that issues the multiplications
+          auto prepare = [&](uint32_t (&v)[32], int first) {
+            if (__builtin_expect(masked, 0)) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (32 * k + i > top || 32 * k + i < bottom) v[32 * k + i] = 0xff800000u;
+                if (first + i > top || first + i < bottom) v[i] = 0xff800000u;
             }
+          };
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          auto look = [&](uint32_t (&v)[32], int first) {
+            prepare(v, first);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(v[32 * k + i]), __uint_as_float(v[32 * k + i + 1]));
+            for (int i = 0; i < 32; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+          };
+#pragma unroll 1
+          for (int k = 0; k < 64; k += 32) {
+            uint32_t v[32];
+            tmem_load32(ts + k, v);
+            tmem_wait_load();
+            look(v, k);
           }
-          const float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * c;
-          const bool grow = mx > m + kSlack;
+          float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]);
+          s_max[x][half][row] = mx;   // the partner has read the one before: its P was awaited before these scores were computed
+          asm volatile("bar.sync %0, 64;" ::"r"(pair_barrier) : "memory");
+          mx = max3(mx, s_max[x][half ^ 1][row], mx) * c;
+          const bool grow = !(mx <= m + kSlack);   // also where the maximum is NaN: so is the reference then, and all of the row
           if (__any_sync(0xffffffffu, grow)) {
             const float m2 = grow ? mx : m, keep = m == -INFINITY ? 0.f : exp2_fast(m - m2);   // nothing seen yet: O and l count for nothing
             m = m2;
             l *= keep;
             if (j > r.first) {   // PV of the block before is done: its completion came with these scores
 #pragma unroll 1
-              for (int d = 0; d < P.dim16; d += 16) {
+              for (int d = o_begin; d < o_end; d += 16) {
                 uint32_t o[16];
                 tmem_load16(to + d, o);
                 tmem_wait_load();
@@ -360,42 +429,49 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const float ref = m == -INFINITY ? 0.f : m;
           const float2 c2 = make_float2(c, c), ref2 = make_float2(-ref, -ref);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          auto weigh = [&](uint32_t (&v)[32], int first) {
+            prepare(v, first);
             uint32_t h[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float2 e = fma2(make_float2(__uint_as_float(v[32 * k + 2 * i]), __uint_as_float(v[32 * k + 2 * i + 1])), c2, ref2);
-              const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+              const float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, ref2);
+              const float2 w = i % kPolyEvery == 1 ? exp2_poly(e) : make_float2(exp2_fast(e.x), exp2_fast(e.y));
               sum[i & 1] = add2(sum[i & 1], w);
               h[i] = pack2<T>(w.x, w.y);
             }
-            tmem_store16(ts + 16 * k, h);
-            if (k == 1) {
-              tmem_wait_store();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(p_half + x);
-            }
+            tmem_store16(ts + first / 2, h);   // over scores that have been read
+          };
+#pragma unroll 1
+          for (int k = 0; k < 64; k += 32) {
+            uint32_t v[32];
+            tmem_load32(ts + k, v);
+            tmem_wait_load();
+            weigh(v, k);
           }
           l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
           tmem_wait_store();
           tc_fence_before();
-        } else if (lane == 0) {
-          mbar_arrive(p_half + x);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + x);
       }
-      if (!ok) break;
-      if (!r.none() && !(ok = t5_wait_warp(o_full + x, o_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+      if (!ok) break;   // of this warp; the others leave at their next wait
+      if (!r.none() && !(ok = wait_warp(o_full + x, o_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
       tc_fence_after();
+      if (leader && !r.none()) mbar_arrive(empty + v_before);
+      if (!idle) {   // the sum of both halves
+        s_max[x][half][row] = l;
+        asm volatile("bar.sync %0, 64;" ::"r"(pair_barrier) : "memory");
+        const float other = s_max[x][half ^ 1][row];
+        l = half ? other + l : l + other;
+        asm volatile("bar.sync %0, 64;" ::"r"(pair_barrier) : "memory");   // before the next block's maximum is put there
+      }
       if (p.begins && p.ends) {
         if (!idle) {
           const float f = 1.f / l;   // 0 only if the row sees nothing
           T* out = static_cast<T*>(P.a.out) + static_cast<long long>(p.s.row0 + p.t0 + x * P.tile_tokens + token) * P.a.out_token +
                    static_cast<long long>(p.h * P.group + head) * P.a.out_head;
-          for (int d = 0; d < P.dim16; d += 16) {
+          for (int d = o_begin; d < o_end; d += 16) {
             uint32_t o[16];
             if (!r.none()) {
               tmem_load16(to + d, o);
@@ -414,10 +490,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       } else if (!idle) {
         float* part = P.partial + (static_cast<size_t>(blockIdx.x) * 4 + (p.begins ? 2 : 0) + x) * tile_partial_floats(P.dim16);
-        part[row] = pos < 0 ? -INFINITY : m;
-        part[128 + row] = pos < 0 ? 0.f : l;
+        if (half == 0) {
+          part[row] = pos < 0 ? -INFINITY : m;
+          part[128 + row] = pos < 0 ? 0.f : l;
+        }
         if (!r.none()) {
-          for (int d = 0; d < P.dim16; d += 16) {
+          for (int d = o_begin; d < o_end; d += 16) {
             uint32_t o[16];
             tmem_load16(to + d, o);
             tmem_wait_load();
@@ -430,7 +508,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       tc_fence_before();   // the next P is announced after these reads of O
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptRegsOther));
     if (warp == 0 || warp == 2) {   // ------------------------------------------------------- loads: warp 0 queries and keys, warp 2 values
       const bool values = warp == 2;
       const void* const map = values ? &VM : &KM;
@@ -441,12 +518,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int per_block = kPosBlock / P.box_rows;   // at most 16
       while (walk.left > 0 && ok) {
         const Piece p = next_piece(P, shape, walk);
+        if (p.j0 == p.j1) continue;
+      if (p.j0 == p.j1) continue;
         const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
         if (!values) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             if (r[x].none() || !ok) continue;
-            if (!(ok = t5_wait_warp(q_empty + x, (q_count[x] & 1) ^ 1, P.wait_limit, P.a.err, abort_flag))) continue;
+            if (!(ok = wait_warp(q_empty + x, (q_count[x] & 1) ^ 1, P.wait_limit, P.a.err, abort_flag))) continue;
             ++q_count[x];
             if (elect_one()) {
               mbar_expect(q_full + x, kHalves * 128u * P.group * P.tile_tokens);
@@ -475,7 +554,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               page = P.a.pool.n_pages;
             }
           }
-          if (!(ok = t5_wait_warp(empty + s, ph ^ 1u, P.wait_limit, P.a.err, abort_flag))) break;
+          if (!(ok = wait_warp(empty + s, ph ^ 1u, P.wait_limit, P.a.err, abort_flag))) break;
           const uint32_t stage = ring + s * Z::kTile;
           const bool cut = values && (end < kPosBlock || begin > 0);
           uint64_t* const bar = cut ? &tail_full : full + s;
@@ -492,7 +571,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
           }
           if (cut) {
-            ok = t5_wait_warp(&tail_full, tails++ & 1, P.wait_limit, P.a.err, abort_flag);
+            ok = wait_warp(&tail_full, tails++ & 1, P.wait_limit, P.a.err, abort_flag);
             uint8_t* dst = smem_raw + (stage - smem_addr(smem_raw));
             for (int n = lane; n < kPosBlock * kHalves * 8; n += 32) {
               const int row = (n >> 3) & 127, half = n >> 10;
@@ -510,91 +589,78 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
         }
       }
-    } else if (warp == 1) {   // ----------------------------------------------------------- multiplications, started by one lane
+    } else {   // ------------------------------------------------ multiplications, started by one lane: warp 1 for the first tile, warp 3 for the second
       constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
-      const uint32_t idesc_s = idesc_f16_m128(kPosBlock) | type, idesc_o = idesc_f16_m128(P.dim16) | type | (1u << 16);   // bit 16: V is position-major
-      const int steps = P.dim16 / 16;
-      int s = 0, q_count[2] = {0, 0}, p_count[2] = {0, 0};
+      const uint32_t idesc_s = idesc_f16_m128(kPosBlock) | type | (P.a.scale < 0.f ? 1u << 13 : 0u), idesc_o = idesc_f16_m128(P.dim16) | type | (1u << 16);   // bit 13: -Q, bit 16: V is position-major
+      const int steps = P.dim16 / 16, x = warp >> 1;
+      const uint32_t ts = tmem + x * 128, to = tmem + 256 + x * 128;
+      const uint64_t q = smem_desc_sw128(base + x * Z::kTile);
+      int s = 0, q_count = 0, p_count = 0;
       uint32_t ph = 0;
-      bool ok = true;
+      bool ok = true, any = false;
       auto wait = [&](uint64_t* bar, int parity) -> bool {
-        if (ok) ok = t5_wait_warp(bar, parity, P.wait_limit, P.a.err, abort_flag);
+        if (ok) ok = wait_warp(bar, parity, P.wait_limit, P.a.err, abort_flag);
         tc_fence_after();
         return ok;
       };
-      auto take = [&](uint32_t& stage) -> bool {   // the next stage of the ring
-        stage = s;
-        wait(full + s, ph);
+      auto next_stage = [&]() -> uint32_t {
+        const uint32_t stage = s;
         if (++s == kStages) {
           s = 0;
           ph ^= 1u;
         }
-        return ok;
-      };
-      auto scores = [&](int x, uint32_t stage, bool last) {
-        const uint64_t q = smem_desc_sw128(base + x * Z::kTile), k = smem_desc_sw128(ring + stage * Z::kTile);
-        if (elect_one()) {
-#pragma unroll
-          for (int i = 0; i < DP / 16; ++i) {   // 32 bytes further inside the swizzle row; then the other half
-            const uint32_t off = (i & 3) * 2 + (i >> 2) * (kHalf >> 4);
-            if (i < steps) mma_ss_f16(tmem + x * 128, q + off, k + off, idesc_s, i > 0);
-          }
-          mma_commit(s_full + x);
-          if (last) mma_commit(q_empty + x);
-        }
-        __syncwarp();
+        return stage;
       };
       while (walk.left > 0 && ok) {
         const Piece p = next_piece(P, shape, walk);
-        const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
-        int j = p.j0;
-        while (j < p.j1 && !r[0].has(j) && !r[1].has(j)) ++j;
-        uint32_t k_stage = 0, v_stage = 0;
-        bool more = j < p.j1;
-        if (more) {   // the first scores
-          if (!take(k_stage)) break;
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            if (r[x].has(j) && wait(q_full + x, q_count[x]++ & 1)) scores(x, k_stage, j + 1 == r[x].last);
-          if (elect_one()) mma_commit(empty + k_stage);
-          __syncwarp();
-        }
-        for (; more && ok; ++j) {
-          more = j + 1 < p.j1 && (r[0].has(j + 1) || r[1].has(j + 1));
-          if (!take(v_stage) || (more && !take(k_stage))) break;
-          const uint64_t v = (smem_desc_sw128(ring + v_stage * Z::kTile) & ~(0x3FFFull << 16)) | (static_cast<uint64_t>(kHalf >> 4) << 16);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (r[x].has(j) && wait(p_half + x, p_count[x] & 1)) {
-              const bool fresh = j == r[x].first, last = j + 1 == r[x].last;
-              if (elect_one()) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)   // 16 positions further: two groups of eight rows
-                  mma_ts_f16(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, v + i * (2048 >> 4), idesc_o, !fresh || i > 0);
-              }
-              __syncwarp();
-              if (wait(p_full + x, p_count[x]++ & 1)) {
-                if (elect_one()) {
-#pragma unroll
-                  for (int i = 4; i < 8; ++i)
-                    mma_ts_f16(tmem + 256 + x * 128, tmem + x * 128 + 8 * i, v + i * (2048 >> 4), idesc_o, true);
-                  if (last) mma_commit(o_full + x);
-                }
-                __syncwarp();
-              }
-            }
-            if (more && r[x].has(j + 1) && (j + 1 > r[x].first || wait(q_full + x, q_count[x]++ & 1)) && ok) scores(x, k_stage, j + 2 == r[x].last);
-          }
+        if (p.j0 == p.j1) continue;
+      if (p.j0 == p.j1) continue;
+        const TileRange r = tile_range(P, p, x), r2 = tile_range(P, p, x ^ 1);
+        uint64_t v = 0;   // the values of the block before
+        for (int j = p.j0; j < p.j1 && ok; ++j) {
+          const bool here = r.has(j);
+          if (!here && !r2.has(j)) continue;
+          const uint32_t k_ph = ph, k_stage = next_stage(), v_ph = ph, v_stage = next_stage();
+          if (!here) continue;   // the other tile's block
+          const bool first = j == r.first, last = j + 1 == r.last;
+          wait(full + k_stage, k_ph);
+          if (first) wait(q_full + x, q_count++ & 1);
+          else wait(p_full + x, p_count++ & 1);
+          if (!ok) break;
+          any = true;
+          const uint64_t k = smem_desc_sw128(ring + k_stage * Z::kTile);
           if (elect_one()) {
-            mma_commit(empty + v_stage);
-            if (more) mma_commit(empty + k_stage);
+            if (!first) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)   // 16 positions further: two groups of eight rows
+                mma_ts_f16(to, ts + 8 * i + (i >> 2) * 32, v + i * (2048 >> 4), idesc_o, j > r.first + 1 || i > 0);
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {   // 32 bytes further inside the swizzle row; then the other half
+              const uint32_t off = (i & 3) * 2 + (i >> 2) * (kHalf >> 4);
+              if (i < steps) mma_ss_f16(ts, q + off, k + off, idesc_s, i > 0);
+            }
+            mma_commit(s_full + x);
           }
           __syncwarp();
+          v = (smem_desc_sw128(ring + v_stage * Z::kTile) & ~(0x3FFFull << 16)) | (static_cast<uint64_t>(kHalf >> 4) << 16);
+          wait(full + v_stage, v_ph);
+          if (last && wait(p_full + x, p_count++ & 1)) {
+            if (elect_one()) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                mma_ts_f16(to, ts + 8 * i + (i >> 2) * 32, v + i * (2048 >> 4), idesc_o, !first || i > 0);
+              mma_commit(o_full + x);
+            }
+            __syncwarp();
+          }
         }
       }
-      if (elect_one()) mma_commit(&mma_done);   // they read shared memory and write tensor memory, which the block is about to give back
-      __syncwarp();
-      if (lane == 0) mbar_wait(smem_addr(&mma_done), 0, P.a.err, 1u << 16);
+      if (any) {
+        if (elect_one()) mma_commit(mma_done + x);   // they read shared memory and write tensor memory, which the block is about to give back
+        __syncwarp();
+        if (lane == 0) mbar_wait(smem_addr(mma_done + x), 0, P.a.err, 1u << 16);
+      }
       __syncwarp();
     }
   }
