@@ -31,10 +31,10 @@
 
 namespace lw {
 
-constexpr int kPromptThreads = 20 * 32;
+constexpr int kPromptThreads = 12 * 32;
+constexpr int kPromptRegsSoftmax = 216, kPromptRegsOther = 72;   // 8 and 4 warps: 12 x 168, the launch's
 constexpr float kSlack = 8.f;
-constexpr int kPolyEvery = 4;
-constexpr int kPromptLead = 2;
+constexpr int kPromptLead = 3;
 
 // The pair that block c continues: its first packed row, rows (tokens) and first query head, and the blocks that hold its first and
 // last unit (first == c: none).  A block leaves the pair that it continues as its piece 0, the one that it only begins as piece 1.
@@ -180,20 +180,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
-// 2^x without the special-function unit, which gives 16 results per cycle and SM where the rest of the softmax could take twice
-// that: x = n + f, n the nearest integer (the rounding of a sum with 1.5 x 2^23), 2^f by a cubic of least relative error over
-// |f| <= 1/2 (7.5e-5, a sixth of half a step of fp16; fitted by reweighted least squares), n added to the exponent.  Below 2^-126:
-// about 2^-126.  A NaN does not come through: a row with one has it in its reference, and the other half of its exponentials.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 shift = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f), minus = make_float2(-1.f, -1.f);
-  const float2 t = add2(x, shift), n = add2(t, back), f = fma2(n, minus, x);
-  float2 p = fma2(f, make_float2(0.05517167f, 0.05517167f), make_float2(0.24261113f, 0.24261113f));
-  p = fma2(p, f, make_float2(0.69326099f, 0.69326099f));
-  p = fma2(p, f, make_float2(0.99992807f, 0.99992807f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
 // The largest of three; a NaN stays
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -220,7 +206,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   __shared__ uint32_t tmem_slot[1];
   __shared__ int abort_word, s_first[4];
   __shared__ long long s_scan[kPromptThreads / 32], s_rest;
-  __shared__ float s_max[2][2][128];   // what the two threads of a row tell each other: [tile][half of the block][row]
   volatile int* abort_flag = &abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_addr(smem_raw), ring = base + 2 * Z::kTile;
@@ -233,7 +218,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(smem_addr(q_full + x), 1);
       mbar_init(smem_addr(q_empty + x), 1);
       mbar_init(smem_addr(s_full + x), 1);
-      mbar_init(smem_addr(p_full + x), 8);
+      mbar_init(smem_addr(p_full + x), 4);
       mbar_init(smem_addr(o_full + x), 1);
       mbar_init(smem_addr(mma_done + x), 1);
     }
@@ -332,15 +317,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   }
 
   if (warp >= 4) {   // -------------------------------------------------------------- softmax
-    // Two threads of a row, in two warps: 64 positions of a block each, and half of the row of O.
-    const int x = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, row = (warp & 3) * 32 + lane, token = row / P.group, head = row - token * P.group;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptRegsSoftmax));
+    const int x = (warp >> 2) - 1, row = (warp & 3) * 32 + lane, token = row / P.group, head = row - token * P.group;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t ts = tmem + lanes + x * 128 + 64 * half, to = tmem + lanes + 256 + x * 128;
-    const int pair_barrier = 1 + x * 4 + (warp & 3);
-    const int o_begin = half ? (P.dim16 / 32) * 16 : 0, o_end = half ? P.dim16 : (P.dim16 / 32) * 16;   // columns of O
+    const uint32_t ts = tmem + lanes + x * 128, to = tmem + lanes + 256 + x * 128;
     // a scale of 0 becomes a very small one: a score hidden as -inf must stay -inf
     const float c = fmaxf(fabsf(P.a.scale) * 1.4426950408889634f, 1e-30f);
-    const bool leading = half == 0 && (warp & 3) == 0, leader = leading && lane == 0;
+    const bool leading = (warp & 3) == 0, leader = leading && lane == 0;
     int s_count = 0, o_count = 0, stage = 0, v_before = 0;
     uint32_t stage_ph = 0;
     bool ok = true;
@@ -381,34 +364,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         v_before = v_stage;
         if (!idle) {
           tc_fence_after();
-          const int p0 = j * kPosBlock, top = pos - p0 - 64 * half, bottom = lo - p0 - 64 * half;
-          const bool masked = p0 + kPosBlock - 1 > r.p_first || (P.a.window > 0 && p0 <= r.p_last - P.a.window);   // some row does not see all of it
-          // S is read twice, for its maximum and for P: the code stays a few KB, which the instruction caches hold beside that of
-          // the warp that issues the multiplications
-          auto prepare = [&](uint32_t (&v)[32], int first) {
-            if (__builtin_expect(masked, 0)) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (first + i > top || first + i < bottom) v[i] = 0xff800000u;
-            }
-          };
+          const int p0 = j * kPosBlock;
+          uint32_t v[128];
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          auto look = [&](uint32_t (&v)[32], int first) {
-            prepare(v, first);
+          tmem_load32(ts, v);
+          tmem_load32(ts + 32, v + 32);
+          tmem_load32(ts + 64, v + 64);
+          tmem_load32(ts + 96, v + 96);
+          tmem_wait_load();
+          if (__builtin_expect(p0 + kPosBlock - 1 > r.p_first || (P.a.window > 0 && p0 <= r.p_last - P.a.window), 0)) {   // some row does not see all of it
+            const int top = pos - p0, bottom = lo - p0;
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-          };
-#pragma unroll 1
-          for (int k = 0; k < 64; k += 32) {
-            uint32_t v[32];
-            tmem_load32(ts + k, v);
-            tmem_wait_load();
-            look(v, k);
+            for (int i = 0; i < 128; ++i)
+              if (i > top || i < bottom) v[i] = 0xff800000u;
           }
-          float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]);
-          s_max[x][half][row] = mx;   // the partner has read the one before: its P was awaited before these scores were computed
-          asm volatile("bar.sync %0, 64;" ::"r"(pair_barrier) : "memory");
-          mx = max3(mx, s_max[x][half ^ 1][row], mx) * c;
+#pragma unroll
+          for (int i = 0; i < 128; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+          const float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * c;
           const bool grow = !(mx <= m + kSlack);   // also where the maximum is NaN: so is the reference then, and all of the row
           if (__any_sync(0xffffffffu, grow)) {
             const float m2 = grow ? mx : m, keep = m == -INFINITY ? 0.f : exp2_fast(m - m2);   // nothing seen yet: O and l count for nothing
@@ -416,7 +388,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             l *= keep;
             if (j > r.first) {   // PV of the block before is done: its completion came with these scores
 #pragma unroll 1
-              for (int d = o_begin; d < o_end; d += 16) {
+              for (int d = 0; d < P.dim16; d += 16) {
                 uint32_t o[16];
                 tmem_load16(to + d, o);
                 tmem_wait_load();
@@ -429,24 +401,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const float ref = m == -INFINITY ? 0.f : m;
           const float2 c2 = make_float2(c, c), ref2 = make_float2(-ref, -ref);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          auto weigh = [&](uint32_t (&v)[32], int first) {
-            prepare(v, first);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
             uint32_t h[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), c2, ref2);
-              const float2 w = i % kPolyEvery == 1 ? exp2_poly(e) : make_float2(exp2_fast(e.x), exp2_fast(e.y));
+              const float2 e = fma2(make_float2(__uint_as_float(v[32 * k + 2 * i]), __uint_as_float(v[32 * k + 2 * i + 1])), c2, ref2);
+              const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
               sum[i & 1] = add2(sum[i & 1], w);
               h[i] = pack2<T>(w.x, w.y);
             }
-            tmem_store16(ts + first / 2, h);   // over scores that have been read
-          };
-#pragma unroll 1
-          for (int k = 0; k < 64; k += 32) {
-            uint32_t v[32];
-            tmem_load32(ts + k, v);
-            tmem_wait_load();
-            weigh(v, k);
+            tmem_store16(ts + 16 * k, h);
           }
           l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
           tmem_wait_store();
@@ -459,19 +424,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (!r.none() && !(ok = wait_warp(o_full + x, o_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
       tc_fence_after();
       if (leader && !r.none()) mbar_arrive(empty + v_before);
-      if (!idle) {   // the sum of both halves
-        s_max[x][half][row] = l;
-        asm volatile("bar.sync %0, 64;" ::"r"(pair_barrier) : "memory");
-        const float other = s_max[x][half ^ 1][row];
-        l = half ? other + l : l + other;
-        asm volatile("bar.sync %0, 64;" ::"r"(pair_barrier) : "memory");   // before the next block's maximum is put there
-      }
       if (p.begins && p.ends) {
         if (!idle) {
           const float f = 1.f / l;   // 0 only if the row sees nothing
           T* out = static_cast<T*>(P.a.out) + static_cast<long long>(p.s.row0 + p.t0 + x * P.tile_tokens + token) * P.a.out_token +
                    static_cast<long long>(p.h * P.group + head) * P.a.out_head;
-          for (int d = o_begin; d < o_end; d += 16) {
+          for (int d = 0; d < P.dim16; d += 16) {
             uint32_t o[16];
             if (!r.none()) {
               tmem_load16(to + d, o);
@@ -490,12 +448,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       } else if (!idle) {
         float* part = P.partial + (static_cast<size_t>(blockIdx.x) * 4 + (p.begins ? 2 : 0) + x) * tile_partial_floats(P.dim16);
-        if (half == 0) {
-          part[row] = pos < 0 ? -INFINITY : m;
-          part[128 + row] = pos < 0 ? 0.f : l;
-        }
+        part[row] = pos < 0 ? -INFINITY : m;
+        part[128 + row] = pos < 0 ? 0.f : l;
         if (!r.none()) {
-          for (int d = o_begin; d < o_end; d += 16) {
+          for (int d = 0; d < P.dim16; d += 16) {
             uint32_t o[16];
             tmem_load16(to + d, o);
             tmem_wait_load();
@@ -508,6 +464,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       tc_fence_before();   // the next P is announced after these reads of O
     }
   } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptRegsOther));
     if (warp == 0 || warp == 2) {   // ------------------------------------------------------- loads: warp 0 queries and keys, warp 2 values
       const bool values = warp == 2;
       const void* const map = values ? &VM : &KM;
@@ -519,7 +476,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       while (walk.left > 0 && ok) {
         const Piece p = next_piece(P, shape, walk);
         if (p.j0 == p.j1) continue;
-      if (p.j0 == p.j1) continue;
         const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
         if (!values) {
 #pragma unroll
@@ -611,12 +567,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
         return stage;
       };
+      uint64_t v = 0;   // the values of the block before
+      auto weighted_sum = [&](bool fresh) {   // O (+)= P V
+        if (!wait(p_full + x, p_count++ & 1)) return;
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)   // 16 positions further: two groups of eight rows
+            mma_ts_f16(to, ts + 8 * i, v + i * (2048 >> 4), idesc_o, !fresh || i > 0);
+        }
+        __syncwarp();
+      };
       while (walk.left > 0 && ok) {
         const Piece p = next_piece(P, shape, walk);
         if (p.j0 == p.j1) continue;
-      if (p.j0 == p.j1) continue;
         const TileRange r = tile_range(P, p, x), r2 = tile_range(P, p, x ^ 1);
-        uint64_t v = 0;   // the values of the block before
         for (int j = p.j0; j < p.j1 && ok; ++j) {
           const bool here = r.has(j);
           if (!here && !r2.has(j)) continue;
@@ -625,16 +589,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const bool first = j == r.first, last = j + 1 == r.last;
           wait(full + k_stage, k_ph);
           if (first) wait(q_full + x, q_count++ & 1);
-          else wait(p_full + x, p_count++ & 1);
+          else weighted_sum(j == r.first + 1);
           if (!ok) break;
           any = true;
           const uint64_t k = smem_desc_sw128(ring + k_stage * Z::kTile);
           if (elect_one()) {
-            if (!first) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)   // 16 positions further: two groups of eight rows
-                mma_ts_f16(to, ts + 8 * i + (i >> 2) * 32, v + i * (2048 >> 4), idesc_o, j > r.first + 1 || i > 0);
-            }
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {   // 32 bytes further inside the swizzle row; then the other half
               const uint32_t off = (i & 3) * 2 + (i >> 2) * (kHalf >> 4);
@@ -645,13 +604,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           __syncwarp();
           v = (smem_desc_sw128(ring + v_stage * Z::kTile) & ~(0x3FFFull << 16)) | (static_cast<uint64_t>(kHalf >> 4) << 16);
           wait(full + v_stage, v_ph);
-          if (last && wait(p_full + x, p_count++ & 1)) {
-            if (elect_one()) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                mma_ts_f16(to, ts + 8 * i + (i >> 2) * 32, v + i * (2048 >> 4), idesc_o, !first || i > 0);
-              mma_commit(o_full + x);
-            }
+          if (last) {
+            weighted_sum(first);
+            if (ok && elect_one()) mma_commit(o_full + x);
             __syncwarp();
           }
         }
