@@ -165,26 +165,20 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, uint32
   return false;
 }
 
-// Two 32-bit operations in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-// The largest of three; a NaN stays
+// The largest of three; NaN are passed over
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+
+__device__ __forceinline__ void tmem_load16_at(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+        "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
 }
 
 template <int DP>
@@ -259,19 +253,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     before = front + inc - v;
     return all;
   };
-  long long units = 0, dummy;
-  for (int b0 = 0; b0 < n_seqs; b0 += kPromptThreads) units += block_sum(seq_units(b0 + tid), dummy);
+  long long units = 0, before = 0, mine_units = 0;
+  for (int b0 = 0; b0 < n_seqs; b0 += kPromptThreads) units += block_sum(mine_units = seq_units(b0 + tid), before);
   const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), units));   // the others have nothing to do
   const long long u0 = static_cast<int>(blockIdx.x) < blocks ? share(units, blockIdx.x, blocks) : 0, u1 = static_cast<int>(blockIdx.x) < blocks ? share(units, blockIdx.x + 1, blocks) : 0;
   if (u0 < u1) {
     long long front = 0;
     for (int b0 = 0; b0 < n_seqs; b0 += kPromptThreads) {
-      const long long mine = seq_units(b0 + tid);
-      long long before;
-      const long long all = block_sum(mine, before);
-      if (u0 >= front + before && u0 < front + before + mine) {
+      long long all = units;
+      if (n_seqs > kPromptThreads) all = block_sum(mine_units = seq_units(b0 + tid), before);
+      if (u0 >= front + before && u0 < front + before + mine_units) {
         const SeqRows s = seq_rows(P, b0 + tid);
-        const long long per_head = mine / P.a.pool.Hk, rest = u0 - front - before;
+        const long long per_head = mine_units / P.a.pool.Hk, rest = u0 - front - before;
         s_first[0] = b0 + tid;
         s_first[1] = static_cast<int>(rest / per_head);
         s_rest = rest % per_head;
@@ -381,7 +374,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
           for (int i = 0; i < 128; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
           const float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * c;
-          const bool grow = !(mx <= m + kSlack);   // also where the maximum is NaN: so is the reference then, and all of the row
+          const bool grow = mx > m + kSlack;
           if (__any_sync(0xffffffffu, grow)) {
             const float m2 = grow ? mx : m, keep = m == -INFINITY ? 0.f : exp2_fast(m - m2);   // nothing seen yet: O and l count for nothing
             m = m2;
@@ -406,9 +399,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             uint32_t h[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float2 e = fma2(make_float2(__uint_as_float(v[32 * k + 2 * i]), __uint_as_float(v[32 * k + 2 * i + 1])), c2, ref2);
+              const float2 e = __ffma2_rn(make_float2(__uint_as_float(v[32 * k + 2 * i]), __uint_as_float(v[32 * k + 2 * i + 1])), c2, ref2);
               const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-              sum[i & 1] = add2(sum[i & 1], w);
+              sum[i & 1] = __fadd2_rn(sum[i & 1], w);
               h[i] = pack2<T>(w.x, w.y);
             }
             tmem_store16(ts + 16 * k, h);
@@ -424,40 +417,36 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (!r.none() && !(ok = wait_warp(o_full + x, o_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
       tc_fence_after();
       if (leader && !r.none()) mbar_arrive(empty + v_before);
-      if (p.begins && p.ends) {
-        if (!idle) {
-          const float f = 1.f / l;   // 0 only if the row sees nothing
-          T* out = static_cast<T*>(P.a.out) + static_cast<long long>(p.s.row0 + p.t0 + x * P.tile_tokens + token) * P.a.out_token +
-                   static_cast<long long>(p.h * P.group + head) * P.a.out_head;
-          for (int d = 0; d < P.dim16; d += 16) {
-            uint32_t o[16];
-            if (!r.none()) {
-              tmem_load16(to + d, o);
-              tmem_wait_load();
-            }
-#pragma unroll
-            for (int k = 0; k < 16; ++k)
-              o[k] = pos < 0 || r.none() ? 0u : __float_as_uint(__uint_as_float(o[k]) * f);
-            if (mine) {
-              auto half8 = [&](int k) { return make_uint4(pack2<T>(__uint_as_float(o[k]), __uint_as_float(o[k + 1])), pack2<T>(__uint_as_float(o[k + 2]), __uint_as_float(o[k + 3])),
-                                                          pack2<T>(__uint_as_float(o[k + 4]), __uint_as_float(o[k + 5])), pack2<T>(__uint_as_float(o[k + 6]), __uint_as_float(o[k + 7]))); };
-              *reinterpret_cast<uint4*>(out + d) = half8(0);
-              if (d + 8 < P.a.pool.Dh) *reinterpret_cast<uint4*>(out + d + 8) = half8(8);
-            }
-          }
-        }
-      } else if (!idle) {
+      if (!idle) {
+        const bool whole = p.begins && p.ends, empty = pos < 0 || r.none();
+        const float f = empty ? 0.f : 1.f / l;
+        T* out = static_cast<T*>(P.a.out) + static_cast<long long>(p.s.row0 + p.t0 + x * P.tile_tokens + token) * P.a.out_token +
+                 static_cast<long long>(p.h * P.group + head) * P.a.out_head;
         float* part = P.partial + (static_cast<size_t>(blockIdx.x) * 4 + (p.begins ? 2 : 0) + x) * tile_partial_floats(P.dim16);
-        part[row] = pos < 0 ? -INFINITY : m;
-        part[128 + row] = pos < 0 ? 0.f : l;
-        if (!r.none()) {
-          for (int d = 0; d < P.dim16; d += 16) {
-            uint32_t o[16];
-            tmem_load16(to + d, o);
+        if (!whole) {
+          part[row] = pos < 0 ? -INFINITY : m;
+          part[128 + row] = pos < 0 ? 0.f : l;
+        }
+#pragma unroll 1
+        for (int d0 = 0; d0 < P.dim16; d0 += 32) {
+          uint32_t o[32];
+          if (!r.none()) {
+            tmem_load16_at(to + d0, o);
+            if (d0 + 16 < P.dim16) tmem_load16_at(to + d0 + 16, o + 16);
             tmem_wait_load();
+          }
+          if (whole) {
 #pragma unroll
-            for (int k = 0; k < 16; k += 4)
-              *reinterpret_cast<uint4*>(part + 256 + (static_cast<size_t>((d + k) / 4) * 128 + row) * 4) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            for (int d = 0; d < 32; d += 8) {
+              uint32_t h[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) h[k] = empty ? 0u : pack2<T>(__uint_as_float(o[d + 2 * k]) * f, __uint_as_float(o[d + 2 * k + 1]) * f);
+              if (mine && d0 + d < P.a.pool.Dh) *reinterpret_cast<uint4*>(out + d0 + d) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+          } else if (!r.none()) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 4)
+              if (d0 + d < P.dim16) *reinterpret_cast<uint4*>(part + 256 + (static_cast<size_t>((d0 + d) / 4) * 128 + row) * 4) = make_uint4(o[d], o[d + 1], o[d + 2], o[d + 3]);
           }
         }
       }
@@ -651,24 +640,33 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
   const size_t tile = tile_partial_floats(P.dim16);
   auto piece = [&](int k) { return P.partial + (static_cast<size_t>(k) * 4 + (k < c ? 2 : 0) + x) * tile; };
   float m = -INFINITY, l = 0.f;
+#pragma unroll 4
   for (int k = c - 1; k <= last; ++k) m = fmaxf(m, piece(k)[row]);
   const float ref = m == -INFINITY ? 0.f : m;
-  for (int k = c - 1; k <= last; ++k) l += piece(k)[128 + row] * exp2_fast(piece(k)[row] - ref);
-  T* out = static_cast<T*>(P.a.out) + static_cast<long long>(n.row0 + t) * P.a.out_token + static_cast<long long>(n.head0 + head) * P.a.out_head;
-  for (int d = warp * 4; d < P.a.pool.Dh; d += kJoinThreads / 32 * 4) {
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = c - 1; k <= last; ++k) {
-      const float* part = piece(k);
-      if (part[128 + row] == 0.f) continue;   // the piece holds nothing for this row, and no O
-      const float f = exp2_fast(part[row] - ref);
-      const float4 v = *reinterpret_cast<const float4*>(part + 256 + (static_cast<size_t>(d / 4) * 128 + row) * 4);
-      o.x = fmaf(f, v.x, o.x);
-      o.y = fmaf(f, v.y, o.y);
-      o.z = fmaf(f, v.z, o.z);
-      o.w = fmaf(f, v.w, o.w);
+  constexpr int kWarps = kJoinThreads / 32, kSteps = 128 / (4 * kWarps);
+  float4 o[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = c - 1; k <= last; ++k) {
+    const float* part = piece(k);
+    const float lk = part[128 + row], f = exp2_fast(part[row] - ref);
+    l += lk * f;
+    if (lk == 0.f) continue;   // the piece holds nothing for this row, and no O
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int d = (i * kWarps + warp) * 4;
+      if (d < P.dim16) {
+        const float4 v = *reinterpret_cast<const float4*>(part + 256 + (static_cast<size_t>(d / 4) * 128 + row) * 4);
+        o[i] = make_float4(fmaf(f, v.x, o[i].x), fmaf(f, v.y, o[i].y), fmaf(f, v.z, o[i].z), fmaf(f, v.w, o[i].w));
+      }
     }
-    const float f = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(o.x * f, o.y * f), pack2<T>(o.z * f, o.w * f));
+  }
+  T* out = static_cast<T*>(P.a.out) + static_cast<long long>(n.row0 + t) * P.a.out_token + static_cast<long long>(n.head0 + head) * P.a.out_head;
+  const float f = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int d = (i * kWarps + warp) * 4;
+    if (d < P.a.pool.Dh) *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(o[i].x * f, o[i].y * f), pack2<T>(o[i].z * f, o[i].w * f));
   }
 }
 
