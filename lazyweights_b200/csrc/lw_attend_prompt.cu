@@ -40,7 +40,7 @@ constexpr int kPromptLead = 3;
 // last unit (first == c: none).  A block leaves the pair that it continues as its piece 0, the one that it only begins as piece 1.
 struct PieceNote {
   int row0, rows, head0, first, last;
-  int pad[3];
+  int b, position, pad;   // its sequence, position of its first token
 };
 
 struct PromptArgs {
@@ -132,6 +132,58 @@ __device__ __forceinline__ TileRange tile_range(const PromptArgs& P, const Piece
   if (r.tokens <= 0 || r.p_last < 0) r.last = r.first = 0;
   return r;
 }
+
+// ---- Values that are not finite.  A tile's rows share the multiplication by V, so an infinite or NaN value of a position reaches
+// the rows of the tile that do not see it too: its weight there is 0, and 0 x inf is NaN.  Where a result is not finite and
+// its sum of weights is, the positions that the tile multiplied but some of its rows do not see are looked through, and if one
+// holds such a value the rows are computed again, one by one (a warp each time; the ordinary path pays a comparison per result).
+
+// The values of position p of kv head kh, this lane's four dimensions; zeros past the head and for a bad page.
+template <typename T>
+__device__ __forceinline__ uint2 four_of(const PromptArgs& P, const void* pool, int b, int kh, int p, int lane) {
+  const int column = p / P.a.pool.page_size, page = P.a.seq.table[b * P.a.seq.table_stride + column];
+  if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(P.a.pool.n_pages) || lane * 4 >= P.a.pool.Dh) return make_uint2(0u, 0u);
+  return *reinterpret_cast<const uint2*>(static_cast<const T*>(pool) + page * P.a.pool.page_stride + kh * P.a.pool.head_stride +
+                                         (p - column * P.a.pool.page_size) * P.a.pool.token_stride + lane * 4);
+}
+template <typename T>
+__device__ __noinline__ bool values_not_finite(const PromptArgs& P, int b, int kh, int from, int to) {
+  constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  const int lane = threadIdx.x & 31;
+  bool bad = false;
+  for (int p = from; p < to; ++p) {
+    const uint2 v = four_of<T>(P, P.a.pool.v, b, kh, p, lane);
+    for (int k = 0; k < 4; ++k) bad |= ((((k & 2) ? v.y : v.x) >> (16 * (k & 1))) & kExponent) == kExponent;
+  }
+  return __any_sync(0xffffffffu, bad);
+}
+// Attention of one row over positions lo .. pos, by a warp.
+template <typename T>
+__device__ __noinline__ void single_row(const PromptArgs& P, int b, int kh, long long row, int head, int lo, int pos) {
+  const int lane = threadIdx.x & 31;
+  auto number = [](uint2 v, int k) {
+    const uint32_t bits = (((k & 2) ? v.y : v.x) >> (16 * (k & 1))) & 0xffffu;
+    const unsigned short u = static_cast<unsigned short>(bits);
+    return static_cast<float>(*reinterpret_cast<const T*>(&u));
+  };
+  const uint2 q = lane * 4 < P.a.pool.Dh ? *reinterpret_cast<const uint2*>(static_cast<const T*>(P.a.q) + row * P.a.q_token + head * P.a.q_head + lane * 4) : make_uint2(0u, 0u);
+  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int p = lo; p <= pos; ++p) {
+    const uint2 k = four_of<T>(P, P.a.pool.k, b, kh, p, lane), v = four_of<T>(P, P.a.pool.v, b, kh, p, lane);
+    float s = 0.f;
+    for (int i = 0; i < 4; ++i) s = fmaf(number(q, i), number(k, i), s);
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    s *= P.a.scale * 1.4426950408889634f;
+    const float m2 = fmaxf(m, s), keep = exp2_fast(m - m2), w = exp2_fast(s - m2);
+    m = m2;
+    l = l * keep + w;
+    for (int i = 0; i < 4; ++i) o[i] = o[i] * keep + w * number(v, i);
+  }
+  if (lane * 4 < P.a.pool.Dh)
+    *reinterpret_cast<uint2*>(static_cast<T*>(P.a.out) + row * P.a.out_token + head * P.a.out_head + lane * 4) =
+        make_uint2(pack2<T>(o[0] / l, o[1] / l), pack2<T>(o[2] / l, o[3] / l));
+}
+__device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= 3.402823466e38f); }
 
 __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* v) {
   asm volatile(
@@ -289,7 +341,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     __syncthreads();
   } else if (tid == 0) {
-    P.notes[blockIdx.x] = {0, 0, 0, static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.x), {0, 0, 0}};
+    P.notes[blockIdx.x] = {0, 0, 0, static_cast<int>(blockIdx.x), static_cast<int>(blockIdx.x), 0, 0, 0};
   }
   Walk walk = {};
   walk.left = u1 - u0;
@@ -305,7 +357,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int t0 = walk.i * shape.pair_tokens, me = blockIdx.x;
       P.notes[me] = {walk.s.row0 + t0, min(shape.pair_tokens, walk.s.q.rows - t0), walk.h * P.group,
                      walk.off > shape.lead ? static_cast<int>(((begin + 1) * blocks - 1) / units) : me,
-                     walk.off > shape.lead ? static_cast<int>(((begin + r.last - r.first) * blocks - 1) / units) : me, {0, 0, 0}};
+                     walk.off > shape.lead ? static_cast<int>(((begin + r.last - r.first) * blocks - 1) / units) : me, walk.b,
+                     walk.s.q.len - walk.s.q.rows + t0, 0};
     }
   }
 
@@ -319,6 +372,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const bool leading = (warp & 3) == 0, leader = leading && lane == 0;
     int s_count = 0, o_count = 0, stage = 0, v_before = 0;
     uint32_t stage_ph = 0;
+    auto mend_rows = [&](const Piece& p, const TileRange& r, bool bad, int pos, int lo, int head, int token) {
+      uint32_t rows = __ballot_sync(0xffffffffu, bad);
+      if (__builtin_expect(rows == 0, 1)) return;
+      const PairRange pr = pair_range(shape, p.s.q, p.t0 / shape.pair_tokens);
+      __syncwarp();
+      if (!values_not_finite<T>(P, p.b, p.h, max(0, r.p_first + 1), pr.hi) &&
+          !(P.a.window > 0 && values_not_finite<T>(P, p.b, p.h, pr.lo, max(0, r.p_last - P.a.window + 1)))) return;
+      for (; rows; rows &= rows - 1) {
+        const int src = __ffs(rows) - 1;
+        const int row_pos = __shfl_sync(0xffffffffu, pos, src), row_lo = __shfl_sync(0xffffffffu, lo, src);
+        single_row<T>(P, p.b, p.h, p.s.row0 + p.t0 + x * P.tile_tokens + __shfl_sync(0xffffffffu, token, src),
+                      p.h * P.group + __shfl_sync(0xffffffffu, head, src), row_lo, row_pos);
+      }
+    };
     bool ok = true;
     while (walk.left > 0 && ok) {
       const Piece p = next_piece(P, shape, walk);
@@ -417,6 +484,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (!r.none() && !(ok = wait_warp(o_full + x, o_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
       tc_fence_after();
       if (leader && !r.none()) mbar_arrive(empty + v_before);
+      float check = 0.f;
       if (!idle) {
         const bool whole = p.begins && p.ends, empty = pos < 0 || r.none();
         const float f = empty ? 0.f : 1.f / l;
@@ -441,7 +509,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               uint32_t h[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k) h[k] = empty ? 0u : pack2<T>(__uint_as_float(o[d + 2 * k]) * f, __uint_as_float(o[d + 2 * k + 1]) * f);
-              if (mine && d0 + d < P.a.pool.Dh) *reinterpret_cast<uint4*>(out + d0 + d) = make_uint4(h[0], h[1], h[2], h[3]);
+              if (mine && d0 + d < P.a.pool.Dh) {
+                *reinterpret_cast<uint4*>(out + d0 + d) = make_uint4(h[0], h[1], h[2], h[3]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) check = fmaf(__uint_as_float(o[d + k]), 0.f, check);   // NaN from the first that is not finite on
+              }
             }
           } else if (!r.none()) {
 #pragma unroll
@@ -450,6 +522,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
         }
       }
+      if (!idle && p.begins && p.ends) mend_rows(p, r, check != 0.f && pos >= 0 && !r.none() && !not_finite(l), pos, lo, head, token);
       tc_fence_before();   // the next P is announced after these reads of O
     }
   } else {
@@ -635,7 +708,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
   const PieceNote n = P.notes[c];
   if (n.first != c - 1) return;   // nothing continued, or not the first to continue it
   const int token = row / P.group, head = row - token * P.group, t = x * P.tile_tokens + token;
-  if (token >= P.tile_tokens || t >= n.rows) return;
+  const bool mine = token < P.tile_tokens && t < n.rows;
   const int last = n.last;
   const size_t tile = tile_partial_floats(P.dim16);
   auto piece = [&](int k) { return P.partial + (static_cast<size_t>(k) * 4 + (k < c ? 2 : 0) + x) * tile; };
@@ -663,10 +736,24 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
   }
   T* out = static_cast<T*>(P.a.out) + static_cast<long long>(n.row0 + t) * P.a.out_token + static_cast<long long>(n.head0 + head) * P.a.out_head;
   const float f = l == 0.f ? 0.f : 1.f / l;
+  bool bad = false;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int d = (i * kWarps + warp) * 4;
-    if (d < P.a.pool.Dh) *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(o[i].x * f, o[i].y * f), pack2<T>(o[i].z * f, o[i].w * f));
+    if (mine && d < P.a.pool.Dh) {
+      *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(o[i].x * f, o[i].y * f), pack2<T>(o[i].z * f, o[i].w * f));
+      bad |= not_finite(o[i].x) || not_finite(o[i].y) || not_finite(o[i].z) || not_finite(o[i].w);
+    }
+  }
+  // as in k_attend_prompt, for all rows of the pair that this warp holds
+  uint32_t rows = __ballot_sync(0xffffffffu, bad && !not_finite(l));
+  if (__builtin_expect(!__syncthreads_or(rows != 0), 1)) return;   // the four warps share the rows, a quarter of the dimensions each
+  const int kh = n.head0 / P.group;
+  if (!values_not_finite<T>(P, n.b, kh, max(0, n.position + 1), n.position + n.rows) &&
+      !(P.a.window > 0 && values_not_finite<T>(P, n.b, kh, max(0, n.position - P.a.window + 1), max(0, n.position + n.rows - P.a.window)))) return;
+  for (; rows; rows &= rows - 1) {   // several warps may write the same row, all of them the same
+    const int src = __ffs(rows) - 1, row_t = __shfl_sync(0xffffffffu, t, src), pos = n.position + row_t;
+    single_row<T>(P, n.b, kh, n.row0 + row_t, n.head0 + __shfl_sync(0xffffffffu, head, src), P.a.window > 0 ? max(0, pos - P.a.window + 1) : 0, pos);
   }
 }
 

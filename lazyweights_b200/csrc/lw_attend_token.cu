@@ -46,6 +46,7 @@ struct TokenArgs {
   int box_rows;             // 16, or 8 where pages are odd multiples of 8
   int cap, least;           // positions the table can name; units of a worker at least, as long as there are fewer than workers
   uint32_t wait_limit, page_inverse;   // floor(2^32 / page size)
+  int drop;                 // a test's lost copy: worker 0 never loads this unit of its share (-1: none)
   TokenNote* notes;         // [worker]
   float* partial;           // [worker][piece]: see TokenSizes
 };
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(kTokenThreads, kTokenBlocksPerSm)
   // ---- loads.  Lane n of the first few starts box n of a unit: keys, then values; half by half of the head dimension; 16 positions
   // in one box or two of eight.  The page of the next unit is asked for when the unit before it is started.
   TokenWalk ahead = at;
-  int load_stage = 0, page = 0, in_page = 0;
+  int load_stage = 0, fills = 0, page = 0, in_page = 0;
   const int per_half = 16 / P.box_rows, boxes = per_half * Z::kHalves;   // of the keys; as many of the values
   const int box_row = (lane % per_half) * P.box_rows, box_half = lane % boxes / per_half;
   const bool loader = lane < 2 * boxes;
@@ -256,13 +257,14 @@ __global__ void __launch_bounds__(kTokenThreads, kTokenBlocksPerSm)
     const int count = __popc(__ballot_sync(0xffffffffu, inside));
     if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count * P.box_rows * 128) : "memory");
     __syncwarp();
-    if (inside) {
+    if (inside && !(P.drop == fills && worker == 0)) {
       if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(P.a.pool.n_pages)) {   // the tensor map's bounds fill it with zeros
         atomicOr(P.a.err, kErrWordIndex);
         page = P.a.pool.n_pages;
       }
       tma_load_4d(box_at + load_stage * 2 * Z::kTile, map, 64 * box_half, in_page, P.chunks == 1 ? ahead.h : ahead.h / P.chunks, page, bar);
     }
+    ++fills;
     if (++load_stage == kStages) load_stage = 0;
     ahead.step(P, slots);
     ask_page();
@@ -322,8 +324,13 @@ __global__ void __launch_bounds__(kTokenThreads, kTokenBlocksPerSm)
 #pragma unroll 1
     for (int t = t_begin; t < t_end; ++t) {
       const int p0 = t * kUnit;
-      (void)mbar_wait(smem_addr(&full[warp][stage]), parity, P.a.err, P.wait_limit);
-      __syncwarp();
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_addr(&full[warp][stage]), parity, P.a.err, P.wait_limit))) {
+        // Given up (the error word says so, the results are void): the copies still in flight land before the warp leaves.
+        if (lane == 0)
+          for (int i = 0; i < kStages; ++i)
+            for (uint32_t turn = 0; turn < 2; ++turn) (void)mbar_wait(smem_addr(&full[warp][i]), turn, P.a.err, 1u << 14);
+        return;
+      }
       const uint32_t at_stage = stage * 2 * Z::kTile;
       // S^T: rows positions, columns heads
       float sc[NT][2][4];
@@ -621,6 +628,7 @@ int launch_attend_token(const PagedCache& cache, const AttendArgs& a, cudaStream
   p.notes = static_cast<TokenNote*>(a.workspace);
   p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + notes_bytes(token_blocks() * kTokenWarps));
   p.least = 2;
+  p.drop = debug_knobs().drop_unit;
   p.page_inverse = static_cast<uint32_t>((1ull << 32) / a.pool.page_size);
   alignas(64) CUtensorMap km, vm;
   const bool half = cache.type == kF16;

@@ -174,6 +174,37 @@ def test_infinities_and_nan_in_sight_show(lw):
     assert torch.isnan(one[0]).all() and torch.isfinite(one[1]).all()
 
 
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("heads,length,new", [(2, 200, 200), (4, 300, 70), (2, 6000, 30)])
+def test_values_out_of_sight_do_not_show(lw, heads, length, new, window):
+    """Infinite and NaN values: they show in the rows that see their position, in their dimension, and nowhere else; also where
+    the rows of one tile see different positions, and where the work on a row is split (the long case)."""
+    import torch
+    from tests import paged_ref as ref
+    pr = problem([length, 100], [new, 100], heads, 1, 64, 16, "fp16", seed=heads)
+    v = ref.load(pr["v"], pr["table"], 0, length)
+    first = length - new
+    places = [(first + new // 2, 3, float("nan")), (length - 1, 5, float("inf")), (first + new // 3, 60, -float("inf")), (max(0, first - 45), 7, float("inf"))]
+    for p, d, x in places:
+        v[p, 0, d] = x
+    ref.store(pr["v"], pr["table"], 0, 0, v)
+    cache = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+    out = cache.attend_prompt(*(pr[n].cuda() for n in ("q", "table", "lens", "starts")), window=window).cpu().double()
+    keys = ref.load(pr["k"], pr["table"], 0, length)
+    clean = torch.where(torch.isfinite(v), v, torch.zeros((), dtype=torch.float64))
+    pos = torch.arange(first, length)
+    want, bound, _ = ref.attend(pr["q"][:new], keys, clean, pos, 64 ** -0.5, window)
+    shows = torch.zeros(new, 64, dtype=torch.bool)
+    for p, d, x in places:
+        shows[:, d] |= (pos >= p) & ((pos - window < p) if window else torch.ones(new, dtype=torch.bool))
+    shows = shows[:, None].expand(new, heads, 64)
+    assert not torch.isfinite(out[:new][shows]).any()
+    assert ((out[:new] - want).abs() <= bound)[~shows].all()
+    assert torch.isfinite(out[new:]).all()
+    one = cache.attend(pr["q"][:2].contiguous().cuda(), pr["table"].cuda(), pr["lens"].cuda(), window=window).cpu()
+    assert torch.equal(~torch.isfinite(one[0]), shows[-1]) and torch.isfinite(one[1]).all()
+
+
 def test_strided_queries_and_results(lw):
     """Queries inside the rows of a fused product, results into a slice of a wider tensor."""
     import torch
@@ -322,6 +353,32 @@ def test_bad_indexes_are_reported(lw):
         assert lw.lib().lw_kernel_error() == 2
         for p in (k, v):
             assert (p[:2, :, 0] == 1).all() and (p[:2, :, 1:] == 5).all() and (p[2] == 5).all()
+
+
+@pytest.mark.parametrize("prompt", [True, False])
+def test_a_lost_copy_ends_the_kernel(lw, prompt):
+    """A copy that never arrives (the kernel's own test switch skips it): the wait for it runs out, the kernel ends, the error word
+    says so, and the next call is right."""
+    import torch
+    # long enough for several units in the share of the first block, or warp, which skips one
+    pr = problem([20000] * 4, [100 if prompt else 1] * 4, 4, 2, 128, 16, "fp16")
+    cache = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+    args = [pr[n].cuda() for n in ("q", "table", "lens")] + ([pr["starts"].cuda()] if prompt else [])
+    call = cache.attend_prompt if prompt else cache.attend
+    want = call(*args)
+    torch.cuda.synchronize()
+    lib = lw.lib()
+    try:
+        for unit in (0, 1):
+            lib.lw_debug_set(b"wait_limit", 2000)
+            lib.lw_debug_set(b"drop_unit", unit)
+            call(*args)
+            torch.cuda.synchronize()
+            assert lib.lw_kernel_error() == 1
+            lib.lw_debug_set(b"reset", 0)
+            assert torch.equal(call(*args), want)
+    finally:
+        lib.lw_debug_set(b"reset", 0)
 
 
 # ------------------------------------------------------------------------------------------- graphs, streams, together
