@@ -94,6 +94,17 @@ int rt_forward(void* handle, const int* ids, int n, float* logits, int all_logit
  * Returns 0, -1 on context overflow, or a negative status. */
 int rt_decode_greedy(void* handle, int first_token, int n, int* out);
 
+/* Several sequences in one pass (additions; the reference's runtime holds one sequence).  rt_pages gives the handle a paged cache of
+ * its own, n_pages pages of page_size positions (a multiple of 8) in every layer, empty; calling it again replaces the cache.
+ * rt_forward_seqs runs the new tokens of n_seqs sequences through the decoder: sequence b's are ids[starts[b]] ..
+ * ids[starts[b + 1] - 1] (starts[0] = 0; one at least per sequence, max_batch at most in all), the last of its lens[b] positions;
+ * its pages are table[b * table_cols + 0 ..], which the caller gives out - two sequences may share the pages of a common
+ * beginning.  logits (host, may be NULL): [n_seqs][vocab], of the last token of every sequence.  All arrays are host arrays, checked before
+ * anything is launched.  The position of rt_forward and its own cache are not touched; rt_set_window applies.  0 or a negative status. */
+int rt_pages(void* handle, int n_pages, int page_size);
+int rt_forward_seqs(void* handle, int n_seqs, const int* ids, const int* starts, const int* lens, const int* table, int table_cols,
+                    float* logits);
+
 void rt_reset(void* handle);
 void rt_set_window(void* handle, int w);
 void rt_set_pos(void* handle, int p);

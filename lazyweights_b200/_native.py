@@ -69,6 +69,8 @@ _SIGNATURES = {
     "lw_ngram_destroy": (None, [C.c_void_p]),
     "lw_ngram_push": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int]),
     "lw_ngram_draft": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int]),
+    "rt_pages": (C.c_int, [C.c_void_p, C.c_int, C.c_int]),
+    "rt_forward_seqs": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
     "lw_cache_create": (C.c_void_p, [C.c_void_p, C.c_void_p] + [C.c_int] * 5 + [C.c_longlong] * 3),
     "lw_cache_destroy": (None, [C.c_void_p]),
     "lw_cache_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,

@@ -22,6 +22,7 @@
 #include "../../include/lwb200.h"
 #include "lw_model.h"
 #include "lw_gemv1.h"
+#include "lw_paged.h"
 
 namespace lw {
 
@@ -103,6 +104,14 @@ struct Runtime {
   std::vector<float*> ln1, ln2;
   std::vector<int> m_qkv, m_q, m_k, m_v, m_o, m_gate, m_up, m_down;
   int m_head = -1;
+  // several sequences with a paged cache (rt_pages, rt_forward_seqs)
+  std::vector<void*> caches;            // one handle per layer
+  int n_pages = 0, page_size = 0;
+  __half *page_pool = nullptr, *q16 = nullptr, *att16 = nullptr;   // every layer's keys, then values; queries and attention of a pass
+  void* attn_space = nullptr;
+  long long attn_space_bytes = 0;
+  int *seq_meta = nullptr, *h_seq_meta = nullptr;   // device and pinned: ids, starts, lens, table of a pass
+  size_t seq_meta_ints = 0;
   std::vector<void*> owned;   // device allocations to free
   std::vector<int> eos;
 };
@@ -313,6 +322,13 @@ __global__ void __launch_bounds__(kNormThreads)
     const float4 g4 = *reinterpret_cast<const float4*>(g + k);
     *reinterpret_cast<float4*>(orow + k) = make_float4(hv.x * r * g4.x, hv.y * r * g4.y, hv.z * r * g4.z, hv.w * r * g4.w);
   }
+}
+
+// rows out[b] = in[starts[b + 1] - 1]: the last token of every sequence
+__global__ void k_last_rows(const float* in, const int* starts, float* __restrict__ out, int D) {
+  dep_begin();
+  const float* src = in + static_cast<size_t>(starts[blockIdx.x + 1] - 1) * D;
+  for (int k = threadIdx.x; k < D; k += blockDim.x) out[static_cast<size_t>(blockIdx.x) * D + k] = src[k];
 }
 
 // rotate-half RoPE on q (in place) and k (into the cache), v into the cache.  grid (heads + 2 kv heads, tokens).
@@ -1087,6 +1103,10 @@ void runtime_free(Model* M) {
     if (R->peer_base[p] && R->peer_base[p] != R->peer_local) cudaIpcCloseMemHandle(R->peer_base[p]);
   if (R->peer_local) cudaFree(R->peer_local);
   if (R->h_ids) cudaFreeHost(R->h_ids);
+  for (void* c : R->caches) lw_cache_destroy(c);
+  if (R->page_pool) cudaFree(R->page_pool);
+  if (R->seq_meta) cudaFree(R->seq_meta);
+  if (R->h_seq_meta) cudaFreeHost(R->h_seq_meta);
   for (void* p : R->owned) cudaFree(p);
   delete R;
   M->rt = nullptr;
@@ -1170,6 +1190,46 @@ static int norm_residual(Model* M, Runtime* R, int m, const float* res, bool res
   return kOk;
 }
 
+// The layer's parts around attention: q, k and v of the normalised rows into R->qkv ...
+static int qkv_products(Model* M, Runtime* R, int l, int m, cudaStream_t st) {
+  const size_t QKV = static_cast<size_t>(R->H + 2 * R->Hk) * R->Dh;
+  int rc = kOk;
+  if (R->m_qkv[l] >= 0) {
+    if ((rc = linear_device(M, M->mats[R->m_qkv[l]], R->xn, false, m, R->qkv, static_cast<int>(QKV), st))) return rc;
+  } else if (m == 1) {   // one token: q, k and v read the same activations - one launch where their plans agree
+    const int idx[3] = {R->m_q[l], R->m_k[l], R->m_v[l]};
+    const float* xs[3] = {R->xn, R->xn, R->xn};
+    float* ys[3] = {R->qkv, R->qkv + R->H * R->Dh, R->qkv + (R->H + R->Hk) * R->Dh};
+    if ((rc = linear_batch_device(M, 3, idx, xs, ys, st))) return rc;
+  } else {
+    if ((rc = linear_device(M, M->mats[R->m_q[l]], R->xn, false, m, R->qkv, static_cast<int>(QKV), st)) ||
+        (rc = linear_device(M, M->mats[R->m_k[l]], R->xn, false, m, R->qkv + R->H * R->Dh, static_cast<int>(QKV), st)) ||
+        (rc = linear_device(M, M->mats[R->m_v[l]], R->xn, false, m, R->qkv + (R->H + R->Hk) * R->Dh,
+                            static_cast<int>(QKV), st)))
+      return rc;
+  }
+  return rc;
+}
+// ... and what follows it: o, the norm, the feed-forward block.  `att`: fp32 or fp16 rows.
+static int rest_of_layer(Model* M, Runtime* R, int l, int m, const void* att, bool att_half, cudaStream_t st) {
+  int rc = kOk;
+  if ((rc = linear_device(M, M->mats[R->m_o[l]], att, att_half, m, R->o, R->D, st))) return rc;
+  if ((rc = norm_residual(M, R, m, R->o, true, R->ln2[l], st, "all-reduce (o)"))) return rc;
+  if (m == 1) {          // one token: gate and up in one launch
+    const int idx[2] = {R->m_gate[l], R->m_up[l]};
+    const float* xs[2] = {R->xn, R->xn};
+    float* ys[2] = {R->g, R->u};
+    if ((rc = linear_batch_device(M, 2, idx, xs, ys, st))) return rc;
+  } else if ((rc = linear_device(M, M->mats[R->m_gate[l]], R->xn, false, m, R->g, R->I, st)) ||
+             (rc = linear_device(M, M->mats[R->m_up[l]], R->xn, false, m, R->u, R->I, st))) {
+    return rc;
+  }
+  const size_t ng = static_cast<size_t>(m) * R->I;
+  launch_dep(k_silu_mul, dim3(static_cast<unsigned>((ng + 255) / 256)), dim3(256), st, R->g, R->u, ng);
+  if ((rc = linear_device(M, M->mats[R->m_down[l]], R->g, false, m, R->o, R->D, st))) return rc;
+  return kOk;
+}
+
 // greedy: the token and the position are already on the device (written by the previous pass's k_argmax_next), and
 // the pass ends with that kernel.
 static int enqueue_pass(Model* M, Runtime* R, int m, bool all_logits, int nchunks, bool cut, cudaStream_t st, bool greedy = false) {
@@ -1179,25 +1239,11 @@ static int enqueue_pass(Model* M, Runtime* R, int m, bool all_logits, int nchunk
   const int* posp = R->ids + R->max_batch;
   if (R->embed16) k_embed16<<<m, 256, 0, st>>>(R->ids, R->embed16, R->h, R->D);
   else k_embed8<<<m, 256, 0, st>>>(R->ids, R->embed8, R->embed_rs, R->embed_rsub, R->h, R->D, R->embed_groups);
-  const size_t QKV = static_cast<size_t>(R->H + 2 * R->Hk) * R->Dh;
   const float* pending = nullptr;   // output of the previous block, added to h by the next norm
   int rc = kOk;
   for (int l = 0; l < R->L; ++l) {
     if ((rc = norm_residual(M, R, m, pending, true, R->ln1[l], st, "all-reduce (down)"))) return rc;
-    if (R->m_qkv[l] >= 0) {
-      if ((rc = linear_device(M, M->mats[R->m_qkv[l]], R->xn, false, m, R->qkv, static_cast<int>(QKV), st))) return rc;
-    } else if (m == 1) {   // one token: q, k and v read the same activations - one launch where their plans agree
-      const int idx[3] = {R->m_q[l], R->m_k[l], R->m_v[l]};
-      const float* xs[3] = {R->xn, R->xn, R->xn};
-      float* ys[3] = {R->qkv, R->qkv + R->H * R->Dh, R->qkv + (R->H + R->Hk) * R->Dh};
-      if ((rc = linear_batch_device(M, 3, idx, xs, ys, st))) return rc;
-    } else {
-      if ((rc = linear_device(M, M->mats[R->m_q[l]], R->xn, false, m, R->qkv, static_cast<int>(QKV), st)) ||
-          (rc = linear_device(M, M->mats[R->m_k[l]], R->xn, false, m, R->qkv + R->H * R->Dh, static_cast<int>(QKV), st)) ||
-          (rc = linear_device(M, M->mats[R->m_v[l]], R->xn, false, m, R->qkv + (R->H + R->Hk) * R->Dh,
-                              static_cast<int>(QKV), st)))
-        return rc;
-    }
+    if ((rc = qkv_products(M, R, l, m, st))) return rc;
     __half* kc = R->kc + static_cast<size_t>(l) * R->Hk * R->Tmax * R->Dh;
     __half* vc = R->vc + static_cast<size_t>(l) * R->Hk * R->Tmax * R->Dh;
     launch_dep(k_rope_cache, dim3(R->H + 2 * R->Hk, m), dim3(64), st, R->qkv, R->cosv, R->sinv, kc, vc, posp, R->H, R->Hk, R->Dh,
@@ -1217,20 +1263,7 @@ static int enqueue_pass(Model* M, Runtime* R, int m, bool all_logits, int nchunk
                    R->max_chunks);
       }
     }
-    if ((rc = linear_device(M, M->mats[R->m_o[l]], R->att, false, m, R->o, R->D, st))) return rc;
-    if ((rc = norm_residual(M, R, m, R->o, true, R->ln2[l], st, "all-reduce (o)"))) return rc;
-    if (m == 1) {          // one token: gate and up in one launch
-      const int idx[2] = {R->m_gate[l], R->m_up[l]};
-      const float* xs[2] = {R->xn, R->xn};
-      float* ys[2] = {R->g, R->u};
-      if ((rc = linear_batch_device(M, 2, idx, xs, ys, st))) return rc;
-    } else if ((rc = linear_device(M, M->mats[R->m_gate[l]], R->xn, false, m, R->g, R->I, st)) ||
-               (rc = linear_device(M, M->mats[R->m_up[l]], R->xn, false, m, R->u, R->I, st))) {
-      return rc;
-    }
-    const size_t ng = static_cast<size_t>(m) * R->I;
-    launch_dep(k_silu_mul, dim3(static_cast<unsigned>((ng + 255) / 256)), dim3(256), st, R->g, R->u, ng);
-    if ((rc = linear_device(M, M->mats[R->m_down[l]], R->g, false, m, R->o, R->D, st))) return rc;
+    if ((rc = rest_of_layer(M, R, l, m, R->att, false, st))) return rc;
     pending = R->o;   // the ranks' partial outputs of `down`: summed by the next norm
   }
   if ((rc = norm_residual(M, R, m, pending, true, R->lnf, st, "all-reduce (down)"))) return rc;
@@ -1253,6 +1286,37 @@ static int enqueue_pass(Model* M, Runtime* R, int m, bool all_logits, int nchunk
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail("forward", e);
   return kOk;
+}
+
+// A pass over the new rows of several sequences with the paged cache (metadata in R->seq_meta): the layers of enqueue_pass
+// with the cache's operators in the place of the runtime's own attention.
+static int enqueue_seqs(Model* M, Runtime* R, int n, int m, int table_cols, bool single, cudaStream_t st) {
+  const int *ids = R->seq_meta, *starts = ids + m, *lens = starts + n + 1, *table = lens + n;
+  if (R->embed16) k_embed16<<<m, 256, 0, st>>>(ids, R->embed16, R->h, R->D);
+  else k_embed8<<<m, 256, 0, st>>>(ids, R->embed8, R->embed_rs, R->embed_rsub, R->h, R->D, R->embed_groups);
+  const int QKV = (R->H + 2 * R->Hk) * R->Dh, row = R->H * R->Dh;
+  const float* pending = nullptr;
+  int rc = kOk;
+  for (int l = 0; l < R->L; ++l) {
+    if ((rc = norm_residual(M, R, m, pending, false, R->ln1[l], st, "norm"))) return rc;
+    if ((rc = qkv_products(M, R, l, m, st))) return rc;
+    if ((rc = lw_cache_append(R->caches[l], R->qkv, LW_TYPE_F32, QKV, m, R->H, R->cosv, R->sinv, R->Tmax, R->Dh / 2, starts, lens, table, n,
+                              table_cols, table_cols, R->q16, row, R->Dh, st)))
+      return rc;
+    if (single)   // a row per sequence
+      rc = lw_cache_attend(R->caches[l], R->q16, row, R->Dh, n, R->H, lens, table, table_cols, table_cols, R->attn_scale, R->window, R->att16, row,
+                           R->Dh, R->attn_space, R->attn_space_bytes, st);
+    else
+      rc = lw_cache_attend_prompt(R->caches[l], R->q16, row, R->Dh, m, R->H, starts, lens, table, n, table_cols, table_cols, R->attn_scale,
+                                  R->window, R->att16, row, R->Dh, R->attn_space, R->attn_space_bytes, st);
+    if (rc || (rc = rest_of_layer(M, R, l, m, R->att16, true, st))) return rc;
+    pending = R->o;
+  }
+  if ((rc = norm_residual(M, R, m, pending, false, R->lnf, st, "norm"))) return rc;
+  launch_dep(k_last_rows, dim3(n), dim3(256), st, R->xn, starts, R->h, R->D);   // h is free from here on
+  if ((rc = linear_device(M, M->mats[R->m_head], R->h, false, n, R->logits, R->V, st))) return rc;
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? kOk : cuda_fail("forward (sequences)", e);
 }
 
 // One pass: direct launches the first time a shape (tokens, context bucket, all_logits) occurs, captured into a CUDA
@@ -1414,6 +1478,107 @@ int rt_forward(void* handle, const int* ids, int n, float* logits, int all_logit
   if (!logits)
     if (const int rcw = guarded_wait(R, "rt_forward")) return rcw;
   return 0;
+}
+
+int rt_pages(void* handle, int n_pages, int page_size) {
+  Model* M = static_cast<Model*>(handle);
+  if (!M || !M->rt || n_pages < 1 || page_size < 8 || page_size % 8 || page_size > 65536) {
+    set_error("rt_pages: no model runtime in this handle, no pages, or a page size that is no multiple of 8");
+    return kErrArg;
+  }
+  Runtime* R = M->rt;
+  if (const int rc = check_device(M)) return rc;
+  if (R->tp_world > 1) {
+    set_error("rt_pages: a tensor-parallel shard serves one sequence");
+    return kErrArg;
+  }
+  cudaStreamSynchronize(R->stream);
+  for (void* c : R->caches) lw_cache_destroy(c);
+  R->caches.clear();
+  if (R->page_pool) cudaFree(R->page_pool);
+  R->page_pool = nullptr;
+  R->n_pages = 0;
+  const size_t page = static_cast<size_t>(R->Hk) * page_size * R->Dh, pool = page * n_pages;
+  cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&R->page_pool), 2 * R->L * pool * sizeof(__half));
+  if (e != cudaSuccess) {
+    R->page_pool = nullptr;
+    cudaGetLastError();
+    return cuda_fail("cudaMalloc (pages)", e);
+  }
+  const long long head = static_cast<long long>(page_size) * R->Dh;
+  for (int l = 0; l < R->L; ++l) {
+    void* c = lw_cache_create(R->page_pool + 2 * l * pool, R->page_pool + (2 * l + 1) * pool, LW_TYPE_F16, n_pages, R->Hk, page_size, R->Dh,
+                              static_cast<long long>(page), head, R->Dh);
+    if (!c) return last_status();
+    R->caches.push_back(c);
+  }
+  const size_t row = static_cast<size_t>(R->max_batch) * R->H * R->Dh;
+  int rc;
+  if (!R->q16 && ((rc = dalloc(R, &R->q16, row)) || (rc = dalloc(R, &R->att16, row)))) return rc;
+  if (!R->attn_space) {
+    for (int prompt = 0; prompt < 2; ++prompt) R->attn_space_bytes = std::max(R->attn_space_bytes, lw_cache_workspace(R->caches[0], R->max_batch, R->H, prompt));
+    uint8_t* space = nullptr;
+    if ((rc = dalloc(R, &space, static_cast<size_t>(R->attn_space_bytes)))) return rc;
+    R->attn_space = space;
+  }
+  R->n_pages = n_pages;
+  R->page_size = page_size;
+  return kOk;
+}
+
+int rt_forward_seqs(void* handle, int n_seqs, const int* ids, const int* starts, const int* lens, const int* table, int table_cols,
+                    float* logits) {
+  Model* M = static_cast<Model*>(handle);
+  auto refuse = [](const char* why) {
+    set_error("rt_forward_seqs: %s", why);
+    return static_cast<int>(kErrArg);
+  };
+  if (!M || !M->rt || !ids || !starts || !lens || !table || n_seqs < 1 || table_cols < 1) return refuse("no model runtime in this handle, or bad argument");
+  Runtime* R = M->rt;
+  if (R->n_pages < 1) return refuse("no pages: call rt_pages first");
+  if (const int rc = check_device(M)) return rc;
+  if (starts[0] != 0) return refuse("the rows begin at 0");
+  bool single = true;
+  for (int b = 0; b < n_seqs; ++b) {
+    const int rows = starts[b + 1] - starts[b];
+    if (rows < 1 || starts[b + 1] > R->max_batch) return refuse("every sequence needs a new token, all of them together at most max_batch");
+    if (lens[b] < rows || lens[b] > R->Tmax) return refuse("a length is less than its new tokens, or beyond the context");
+    const int pages = (lens[b] + R->page_size - 1) / R->page_size;
+    if (pages > table_cols) return refuse("the page table has too few columns for a length");
+    for (int k = 0; k < pages; ++k)
+      if (table[static_cast<size_t>(b) * table_cols + k] < 0 || table[static_cast<size_t>(b) * table_cols + k] >= R->n_pages) return refuse("a page index is outside the pool");
+    single = single && rows == 1;
+  }
+  const int m = starts[n_seqs];
+  for (int i = 0; i < m; ++i)
+    if (ids[i] < 0 || ids[i] >= R->embed_rows) return refuse("a token id is outside the embedding");
+  cudaStream_t st = R->stream;
+  cudaError_t e = cudaStreamSynchronize(st);   // the pinned buffer is reused
+  if (e != cudaSuccess) return cuda_fail("rt_forward_seqs", e);
+  const size_t ints = static_cast<size_t>(m) + 2 * n_seqs + 1 + static_cast<size_t>(n_seqs) * table_cols;
+  if (ints > R->seq_meta_ints) {
+    if (R->seq_meta) cudaFree(R->seq_meta);
+    if (R->h_seq_meta) cudaFreeHost(R->h_seq_meta);
+    R->seq_meta = R->h_seq_meta = nullptr;
+    R->seq_meta_ints = 0;
+    if ((e = cudaMalloc(reinterpret_cast<void**>(&R->seq_meta), 2 * ints * sizeof(int))) != cudaSuccess ||
+        (e = cudaMallocHost(reinterpret_cast<void**>(&R->h_seq_meta), 2 * ints * sizeof(int))) != cudaSuccess) {
+      cudaGetLastError();
+      return cuda_fail("rt_forward_seqs", e);
+    }
+    R->seq_meta_ints = 2 * ints;
+  }
+  int* at = R->h_seq_meta;
+  std::memcpy(at, ids, m * sizeof(int));
+  std::memcpy(at += m, starts, (n_seqs + 1) * sizeof(int));
+  std::memcpy(at += n_seqs + 1, lens, n_seqs * sizeof(int));
+  std::memcpy(at += n_seqs, table, static_cast<size_t>(n_seqs) * table_cols * sizeof(int));
+  e = cudaMemcpyAsync(R->seq_meta, R->h_seq_meta, ints * sizeof(int), cudaMemcpyHostToDevice, st);
+  if (e != cudaSuccess) return cuda_fail("rt_forward_seqs", e);
+  if (const int rc = enqueue_seqs(M, R, n_seqs, m, table_cols, single, st)) return rc;
+  if (logits) e = cudaMemcpyAsync(logits, R->logits, static_cast<size_t>(n_seqs) * R->V * sizeof(float), cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  return e == cudaSuccess ? kOk : cuda_fail("rt_forward_seqs", e);
 }
 
 int rt_decode_greedy(void* handle, int first_token, int n, int* out) {

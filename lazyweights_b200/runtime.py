@@ -255,6 +255,25 @@ class Bundle(_Handle):
         nat.check(rc)
         return out
 
+    def open_pages(self, n_pages, page_size=16):
+        """rt_pages: a paged cache for several sequences, `n_pages` pages of `page_size` positions in every layer."""
+        nat.check(nat.lib().rt_pages(self._h, int(n_pages), int(page_size)))
+
+    def forward_seqs(self, ids, lens, table):
+        """rt_forward_seqs: one pass over the new tokens of several sequences.  ids: a list of their token arrays, lens: their lengths
+        with the new tokens, table: [n, columns] their pages.  Returns the logits of every sequence's last token [n, vocab] (host
+        float32)."""
+        parts = [np.ascontiguousarray(i, np.int32).reshape(-1) for i in ids]
+        starts = np.cumsum([0] + [p.size for p in parts]).astype(np.int32)
+        flat = np.concatenate(parts) if parts else np.zeros(0, np.int32)
+        lens, table = np.ascontiguousarray(lens, np.int32).reshape(-1), np.ascontiguousarray(table, np.int32)
+        if table.ndim != 2 or table.shape[0] != len(parts) or lens.size != len(parts):
+            raise ValueError("forward_seqs wants a length and a row of the page table per sequence")
+        out = np.empty((len(parts), nat.lib().rt_vocab(self._h)), np.float32)
+        nat.check(nat.lib().rt_forward_seqs(self._h, len(parts), flat.ctypes.data, starts.ctypes.data, lens.ctypes.data, table.ctypes.data,
+                                            table.shape[1], out.ctypes.data))
+        return out
+
     def decode_greedy(self, first_token, n):
         """rt_decode_greedy: n greedy one-token passes without a host round trip per token; returns the n chosen tokens
         (int32).  The same tokens as n calls of forward() with np.argmax in between."""
