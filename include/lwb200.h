@@ -324,10 +324,9 @@ int lw_cache_append(void* cache, const void* qkv, int qkv_type, long long row_st
                     int n_seqs, int table_cols, long long table_stride, void* q, long long q_token_stride, long long q_head_stride,
                     void* stream);
 
-/* Bytes of workspace that attention over n_rows rows of n_heads heads needs (0: none, a null workspace will do); prompt: of
- * lw_cache_attend_prompt.  The caller owns it, on a 16-byte boundary; its contents do not matter.  Calls that overlap on the
+/* Bytes of workspace that attention of n_heads heads needs, whatever the rows and lengths; prompt: of lw_cache_attend_prompt.  The caller owns it, on a 16-byte boundary; its contents do not matter.  Calls that overlap on the
  * GPU - captured ones too - need one each. */
-long long lw_cache_workspace(void* cache, int n_rows, int n_heads, int prompt);
+long long lw_cache_workspace(void* cache, int n_heads, int prompt);
 
 /* Attention of one new token per sequence: out[b][h] = sum_j softmax_j(scale q[b][h] . k_j) v_j over the positions
  * max(0, lens[b] - window) <= j < lens[b] (window 0: from 0).  Query head h reads kv head h / (n_heads / n_kv_heads).  q and out in

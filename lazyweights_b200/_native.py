@@ -76,7 +76,7 @@ _SIGNATURES = {
     "lw_cache_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int,
                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_longlong, C.c_void_p, C.c_longlong,
                                   C.c_longlong, C.c_void_p]),
-    "lw_cache_workspace": (C.c_longlong, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
+    "lw_cache_workspace": (C.c_longlong, [C.c_void_p, C.c_int, C.c_int]),
     "lw_cache_attend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_longlong, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
                                   C.c_longlong, C.c_float, C.c_int, C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p, C.c_longlong,
                                   C.c_void_p]),

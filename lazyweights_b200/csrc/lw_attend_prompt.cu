@@ -647,7 +647,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const bool here = r.has(j);
           if (!here && !r2.has(j)) continue;
           const uint32_t k_ph = ph, k_stage = next_stage(), v_ph = ph, v_stage = next_stage();
-          if (!here) continue;   // the other tile's block
+          if (!here) {   // the other tile's block: waited for all the same, a barrier's parity tells only neighbouring turns of a stage apart
+            wait(full + k_stage, k_ph);
+            wait(full + v_stage, v_ph);
+            continue;
+          }
           const bool first = j == r.first, last = j + 1 == r.last;
           wait(full + k_stage, k_ph);
           if (first) wait(q_full + x, q_count++ & 1);
@@ -803,22 +807,21 @@ int launch_attend_prompt(const PagedCache& cache, const AttendArgs& a, cudaStrea
   p.a = a;
   p.group = a.H / a.pool.Hk;
   p.tile_tokens = 128 / p.group;
-  p.box_rows = std::min(kPosBlock, a.pool.page_size & -a.pool.page_size);
+  p.box_rows = cache.prompt_rows;
   p.dim16 = (a.pool.Dh + 15) / 16 * 16;
   p.cap = static_cast<int>(std::min<long long>(static_cast<long long>(a.seq.table_cols) * a.pool.page_size, 1 << 30));
   p.wait_limit = debug_knobs().wait_limit;
   p.drop = debug_knobs().drop_unit;
   p.notes = static_cast<PieceNote*>(a.workspace);
   p.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + notes_bytes(sm_count()));
-  alignas(64) CUtensorMap qm, km, vm;
+  alignas(64) CUtensorMap qm;
   const bool half = cache.type == kF16;
-  if (!make_query_map(&qm, half, a.q, a.pool.Dh, a.H, a.rows, a.q_head, a.q_token, p.group, p.tile_tokens) ||
-      !make_page_map(&km, half, a.pool.k, a.pool, p.box_rows) || !make_page_map(&vm, half, a.pool.v, a.pool, p.box_rows)) {
-    set_kernel_error_text("attend_prompt", "the driver refused a tensor map over the queries or the pages");
+  if (!make_query_map(&qm, half, a.q, a.pool.Dh, a.H, a.rows, a.q_head, a.q_token, p.group, p.tile_tokens)) {
+    set_kernel_error_text("attend_prompt", "the driver refused a tensor map over the queries");
     return kErrArg;
   }
-  if (a.pool.Dh <= 64) return half ? launch<__half, 64>(qm, km, vm, p, st) : launch<__nv_bfloat16, 64>(qm, km, vm, p, st);
-  return half ? launch<__half, 128>(qm, km, vm, p, st) : launch<__nv_bfloat16, 128>(qm, km, vm, p, st);
+  if (a.pool.Dh <= 64) return half ? launch<__half, 64>(qm, cache.prompt_k, cache.prompt_v, p, st) : launch<__nv_bfloat16, 64>(qm, cache.prompt_k, cache.prompt_v, p, st);
+  return half ? launch<__half, 128>(qm, cache.prompt_k, cache.prompt_v, p, st) : launch<__nv_bfloat16, 128>(qm, cache.prompt_k, cache.prompt_v, p, st);
 }
 
 }  // namespace lw

@@ -622,7 +622,7 @@ int launch_attend_token(const PagedCache& cache, const AttendArgs& a, cudaStream
   p.a = a;
   p.group = a.H / a.pool.Hk;
   p.chunks = (p.group + 15) / 16;
-  p.box_rows = a.pool.page_size % 16 ? 8 : 16;
+  p.box_rows = cache.token_rows;
   p.cap = static_cast<int>(std::min<long long>(static_cast<long long>(a.seq.table_cols) * a.pool.page_size, 1 << 30));
   p.wait_limit = debug_knobs().wait_limit;
   p.notes = static_cast<TokenNote*>(a.workspace);
@@ -630,13 +630,8 @@ int launch_attend_token(const PagedCache& cache, const AttendArgs& a, cudaStream
   p.least = 2;
   p.drop = debug_knobs().drop_unit;
   p.page_inverse = static_cast<uint32_t>((1ull << 32) / a.pool.page_size);
-  alignas(64) CUtensorMap km, vm;
-  const bool half = cache.type == kF16;
-  if (!make_page_map(&km, half, a.pool.k, a.pool, p.box_rows) || !make_page_map(&vm, half, a.pool.v, a.pool, p.box_rows)) {
-    set_kernel_error_text("attend", "the driver refused a tensor map over the pages");
-    return kErrArg;
-  }
-  return half ? launch_type<__half>(km, vm, p, st) : launch_type<__nv_bfloat16>(km, vm, p, st);
+  const CUtensorMap &km = cache.token_k, &vm = cache.token_v;
+  return cache.type == kF16 ? launch_type<__half>(km, vm, p, st) : launch_type<__nv_bfloat16>(km, vm, p, st);
 }
 
 }  // namespace lw

@@ -1,6 +1,7 @@
 // The paged key-value cache: its handle, the kernel that appends rotated keys and values, the C entry points.
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <new>
@@ -188,10 +189,9 @@ static bool aligned(const void* p, unsigned int bytes) { return (reinterpret_cas
 
 // The current device, if it is the cache's.
 static int check_cache_device(const PagedCache* c) {
-  int n = 0, dev = -1;
-  if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
-    cudaGetLastError();
-    set_error("no CUDA device: this library has no CPU path for GPU entry points");
+  int dev = -1;
+  if (c->device < 0) {
+    set_error("the cache was created without a CUDA device: this library has no CPU path for GPU entry points");
     return kErrNoDevice;
   }
   if (cudaGetDevice(&dev) != cudaSuccess) return cuda_fail("cudaGetDevice", cudaGetLastError());
@@ -262,6 +262,15 @@ void* lw_cache_create(void* k_pages, void* v_pages, int type, int n_pages, int n
     cudaGetLastError();
     c->device = -1;
   }
+  c->token_rows = page_size % 16 ? 8 : 16;
+  c->prompt_rows = std::min(128, page_size & -page_size);
+  const bool half = type == kF16;
+  if (c->device >= 0 && !(make_page_map(&c->token_k, half, k_pages, c->pool, c->token_rows) && make_page_map(&c->token_v, half, v_pages, c->pool, c->token_rows) &&
+                          make_page_map(&c->prompt_k, half, k_pages, c->pool, c->prompt_rows) && make_page_map(&c->prompt_v, half, v_pages, c->pool, c->prompt_rows))) {
+    delete c;
+    note_status(refuse(what, "the driver refused a tensor map over the pools"));
+    return nullptr;
+  }
   note_status(kOk);
   return c;
 }
@@ -319,7 +328,7 @@ static int attend(const char* what, void* cache, const void* q, long long q_toke
   if (const int rc = check_rows(what, out, out_token_stride, out_head_stride, n_heads, c->pool.Dh, n_rows)) return rc;
   if (n_heads / c->pool.Hk > 128) return refuse(what, "at most 128 query heads per kv head");
   if (!std::isfinite(scale) || window < 0) return refuse(what, "the scale must be finite, the window not negative");
-  const long long need = lw_cache_workspace(cache, n_rows, n_heads, prompt);
+  const long long need = lw_cache_workspace(cache, n_heads, prompt);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return refuse(what, "the workspace is too small (lw_cache_workspace), or not on a 16-byte boundary");
   if (const int rc = check_cache_device(c)) return rc;
@@ -341,9 +350,9 @@ static int attend(const char* what, void* cache, const void* q, long long q_toke
   return (prompt ? launch_attend_prompt : launch_attend_token)(*c, a, static_cast<cudaStream_t>(stream));
 }
 
-long long lw_cache_workspace(void* cache, int n_rows, int n_heads, int prompt) {
+long long lw_cache_workspace(void* cache, int n_heads, int prompt) {
   const PagedCache* c = static_cast<const PagedCache*>(cache);
-  if (!c || n_rows < 1 || n_heads < 1 || n_heads % c->pool.Hk) return refuse("lw_cache_workspace", "bad argument");
+  if (!c || n_heads < 1 || n_heads % c->pool.Hk) return refuse("lw_cache_workspace", "bad argument");
   return prompt ? prompt_workspace(c->pool.Dh) : token_workspace(c->pool.Dh, n_heads / c->pool.Hk);
 }
 

@@ -24,6 +24,9 @@ struct PagedCache {
   PagePool pool;
   ElemType type;
   int device = -1;   // -1: made without a CUDA device; nothing can be launched on it
+  // Positions of a TMA box, a divisor of the page size: of 16 at a time (one token), of 128 (prompts); the maps of keys and values.
+  int token_rows, prompt_rows;
+  alignas(64) CUtensorMap token_k, token_v, prompt_k, prompt_v;
 };
 
 // Which positions belong to which rows: sequence b owns rows starts[b] .. starts[b + 1] - 1 (row b alone if starts is null),

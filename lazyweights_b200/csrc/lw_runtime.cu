@@ -1516,7 +1516,7 @@ int rt_pages(void* handle, int n_pages, int page_size) {
   int rc;
   if (!R->q16 && ((rc = dalloc(R, &R->q16, row)) || (rc = dalloc(R, &R->att16, row)))) return rc;
   if (!R->attn_space) {
-    for (int prompt = 0; prompt < 2; ++prompt) R->attn_space_bytes = std::max(R->attn_space_bytes, lw_cache_workspace(R->caches[0], R->max_batch, R->H, prompt));
+    for (int prompt = 0; prompt < 2; ++prompt) R->attn_space_bytes = std::max(R->attn_space_bytes, lw_cache_workspace(R->caches[0], R->H, prompt));
     uint8_t* space = nullptr;
     if ((rc = dalloc(R, &space, static_cast<size_t>(R->attn_space_bytes)))) return rc;
     R->attn_space = space;

@@ -31,7 +31,7 @@ class PagedCache:
 
     def __init__(self, k_pages, v_pages):
         torch = _torch()
-        self._h = None
+        self._h, self._spaces = None, {}
         if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype is not v_pages.dtype or \
                 k_pages.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError("PagedCache wants two fp16 or bf16 pools [pages, kv_heads, page_size, head_dim] of one shape and type")
@@ -124,9 +124,12 @@ class PagedCache:
             nat.check(rc)
         return q
 
-    def _workspace(self, torch, rows, heads, prompt):
-        need = nat.check(nat.lib().lw_cache_workspace(self._h, rows, heads, prompt))
-        return torch.empty(need, dtype=torch.uint8, device=self.device) if need else None, need
+    def _workspace(self, torch, heads, prompt):
+        """A workspace of the call's own: calls may overlap, and captured ones too."""
+        need = self._spaces.get((heads, prompt))
+        if need is None:
+            need = self._spaces[heads, prompt] = nat.check(nat.lib().lw_cache_workspace(self._h, heads, prompt))
+        return torch.empty(need, dtype=torch.uint8, device=self.device), need
 
     def attend(self, q, table, lens, scale=None, window=0, out=None):
         """Attention of one new token per sequence: q [n, heads, head_dim] -> the same shape (`out`: a tensor to fill).  scale: of
@@ -138,10 +141,10 @@ class PagedCache:
         if out is None:
             out = torch.empty((n, q.shape[1], self.head_dim), dtype=self.dtype, device=self.device)
         ot, oh = self._rows(out, "out", n, q.shape[1])
-        space, size = self._workspace(torch, n, q.shape[1], 0)
+        space, size = self._workspace(torch, q.shape[1], 0)
         rc = nat.lib().lw_cache_attend(self._h, q.data_ptr(), qt, qh, n, q.shape[1], lens.data_ptr(), table.data_ptr(), cols, tstride,
                                        self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(), ot, oh,
-                                       space.data_ptr() if size else None, size, _stream(torch, self._index))
+                                       space.data_ptr(), size, _stream(torch, self._index))
         if rc < 0:
             nat.check(rc)
         return out
@@ -158,10 +161,10 @@ class PagedCache:
         if out is None:
             out = torch.empty((rows, heads, self.head_dim), dtype=self.dtype, device=self.device)
         ot, oh = self._rows(out, "out", rows, heads)
-        space, size = self._workspace(torch, rows, heads, 1)
+        space, size = self._workspace(torch, heads, 1)
         rc = nat.lib().lw_cache_attend_prompt(self._h, q.data_ptr(), qt, qh, rows, heads, starts.data_ptr(), lens.data_ptr(), table.data_ptr(),
                                               n, cols, tstride, self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
-                                              ot, oh, space.data_ptr() if size else None, size, _stream(torch, self._index))
+                                              ot, oh, space.data_ptr(), size, _stream(torch, self._index))
         if rc < 0:
             nat.check(rc)
         return out

@@ -112,6 +112,15 @@ def test_prompts_few_and_many(lw, lens, heads, kv_heads):
     check_attention(lw, problem([n for n, _ in lens], [m for _, m in lens], heads, kv_heads, 128, 16, "bf16", seed=len(lens), gap=1))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [0, 300])
+def test_pairs_whose_second_tile_is_empty(lw, dim, window):
+    """Prompts that end inside the first tile of a pair of tiles, so that the second one passes over more position blocks than the
+    stages hold, between pairs that need both; several of them per block of the grid."""
+    lens = [1055, 1055, 700, 33, 1055, 1090, 1055, 33, 1055, 1055]
+    check_attention(lw, problem(lens, lens, 16, 8, dim, 16, "fp16", seed=dim), window=window)
+
+
 @pytest.mark.parametrize("window", [1, 2, 17, 64, 127, 128, 129, 500, 100000])
 def test_prompt_window(lw, window):
     lens = [(1, 1), (70, 70), (300, 200), (128, 128), (900, 40), (1030, 1030)]

@@ -87,14 +87,13 @@ def test_a_workspace_too_small_is_refused(nat):
     h = create(nat)
     try:
         for prompt, fn, base in ((0, "lw_cache_attend", ATTEND), (1, "lw_cache_attend_prompt", PROMPT)):
-            need = nat.lib().lw_cache_workspace(h, base["rows"], base["heads"], prompt)
-            assert need >= 0
-            if need:
-                for kw in (dict(size=need - 1), dict(space=None), dict(space=P + 8)):
-                    assert getattr(nat.lib(), fn)(h, *dict(base, **kw).values()) == nat.LW_ERR_ARG
-        for bad in ((0, 8, 0), (3, 0, 0), (3, 6, 1)):
+            need = nat.lib().lw_cache_workspace(h, base["heads"], prompt)
+            assert need > 0
+            for kw in (dict(size=need - 1), dict(space=None), dict(space=P + 8)):
+                assert getattr(nat.lib(), fn)(h, *dict(base, **kw).values()) == nat.LW_ERR_ARG
+        for bad in ((0, 0), (6, 1), (-4, 0)):
             assert nat.lib().lw_cache_workspace(h, *bad) == nat.LW_ERR_ARG
-        assert nat.lib().lw_cache_workspace(None, 1, 8, 0) == nat.LW_ERR_ARG
+        assert nat.lib().lw_cache_workspace(None, 8, 0) == nat.LW_ERR_ARG
     finally:
         nat.lib().lw_cache_destroy(h)
 
