@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   constexpr int kStages = Z::kStages;
   constexpr uint32_t kHalf = 128 * 128;   // bytes of 64 columns of a tile: 128 rows of 128 bytes, swizzled
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], mma_done[2], tail_full;
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[2], s_full[2], p_full[2], o_full[2], mma_done[2], tail_full;
   __shared__ uint32_t tmem_slot[1];
   __shared__ int abort_word, s_first[4];
   __shared__ long long s_scan[kPromptThreads / 32], s_rest;
@@ -262,7 +262,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(smem_addr(q_full + x), 1);
-      mbar_init(smem_addr(q_empty + x), 1);
       mbar_init(smem_addr(s_full + x), 1);
       mbar_init(smem_addr(p_full + x), 4);
       mbar_init(smem_addr(o_full + x), 1);
@@ -369,9 +368,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const uint32_t ts = tmem + lanes + x * 128, to = tmem + lanes + 256 + x * 128;
     // a scale of 0 becomes a very small one: a score hidden as -inf must stay -inf
     const float c = fmaxf(fabsf(P.a.scale) * 1.4426950408889634f, 1e-30f);
-    const bool leading = (warp & 3) == 0, leader = leading && lane == 0;
+    const bool leader = (warp & 3) == 0 && lane == 0;
     int s_count = 0, o_count = 0, stage = 0, v_before = 0;
-    uint32_t stage_ph = 0;
     auto mend_rows = [&](const Piece& p, const TileRange& r, bool bad, int pos, int lo, int head, int token) {
       uint32_t rows = __ballot_sync(0xffffffffu, bad);
       if (__builtin_expect(rows == 0, 1)) return;
@@ -402,24 +400,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         // The scores' completion tells that the multiplications are done with the keys of this block and the values of the one
         // before: one thread per tile gives the stages back.  (A commit of its own for each would hold the tensor core up by 78 cycles.)
         const int k_stage = stage, v_stage = k_stage + 1 == kStages ? 0 : k_stage + 1;
-        const uint32_t k_ph = stage_ph, v_ph = k_ph ^ (v_stage == 0 ? 1u : 0u);
         stage = v_stage + 1 == kStages ? 0 : v_stage + 1;
-        stage_ph = v_ph ^ (stage == 0 ? 1u : 0u);
-        if (!here) {   // the other tile's: given back once it is there, so that the turns of a stage stay apart
-          if (leading) {
-            if (!(ok = wait_warp(full + k_stage, k_ph, P.wait_limit, P.a.err, abort_flag) && wait_warp(full + v_stage, v_ph, P.wait_limit, P.a.err, abort_flag))) break;
-            if (leader) {
-              mbar_arrive(empty + k_stage);
-              mbar_arrive(empty + v_stage);
-            }
-          }
-          continue;
-        }
+        if (!here) continue;   // the other tile's; this tile's issuing warp gives the stages back
         if (!(ok = wait_warp(s_full + x, s_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
         if (leader) {
           mbar_arrive(empty + k_stage);
           if (j > r.first) mbar_arrive(empty + v_before);
-          if (j + 1 == r.last) mbar_arrive(q_empty + x);
         }
         v_before = v_stage;
         if (!idle) {
@@ -527,10 +513,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptRegsOther));
-    if (warp == 0 || warp == 2) {   // ------------------------------------------------------- loads: warp 0 queries and keys, warp 2 values
+    if (warp == 0 || warp == 2) {   // ------------------------------------------------------- loads: warp 0 keys, warp 2 values
       const bool values = warp == 2;
       const void* const map = values ? &VM : &KM;
-      int s = values, q_count[2] = {0, 0}, tails = 0, fills = 0;
+      int s = values, tails = 0, fills = 0;
       uint32_t ph = 0;
       bool ok = true;
       constexpr int kHalves = DP / 64;
@@ -539,21 +525,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const Piece p = next_piece(P, shape, walk);
         if (p.j0 == p.j1) continue;
         const TileRange r[2] = {tile_range(P, p, 0), tile_range(P, p, 1)};
-        if (!values) {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (r[x].none() || !ok) continue;
-            if (!(ok = wait_warp(q_empty + x, (q_count[x] & 1) ^ 1, P.wait_limit, P.a.err, abort_flag))) continue;
-            ++q_count[x];
-            if (elect_one()) {
-              mbar_expect(q_full + x, kHalves * 128u * P.group * P.tile_tokens);
-#pragma unroll
-              for (int d = 0; d < kHalves; ++d)
-                tma_load_3d(base + x * Z::kTile + d * kHalf, &QM, 64 * d, p.h * P.group, p.s.row0 + p.t0 + x * P.tile_tokens, smem_addr(q_full + x));
-            }
-            __syncwarp();
-          }
-        }
         // positions that some row of the pair sees
         const PairRange pr = pair_range(shape, p.s.q, p.t0 / shape.pair_tokens);
         const int* table = P.a.seq.table + p.b * P.a.seq.table_stride;
@@ -647,15 +618,32 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const bool here = r.has(j);
           if (!here && !r2.has(j)) continue;
           const uint32_t k_ph = ph, k_stage = next_stage(), v_ph = ph, v_stage = next_stage();
-          if (!here) {   // the other tile's block: waited for all the same, a barrier's parity tells only neighbouring turns of a stage apart
+          if (!here) {
+            // The other tile's block, given back once it is there: the turns of a stage must not overtake a warp that waits on its
+            // barriers, whose parity tells only neighbouring turns apart.
             wait(full + k_stage, k_ph);
-            wait(full + v_stage, v_ph);
+            if (wait(full + v_stage, v_ph) && elect_one()) {
+              mbar_arrive(empty + k_stage);
+              mbar_arrive(empty + v_stage);
+            }
+            __syncwarp();
             continue;
           }
           const bool first = j == r.first, last = j + 1 == r.last;
+          if (first) {
+            // This tile's queries.  The multiplications that read the last ones are done: their scores have become the P of the last
+            // weighted sum.  The latency passes while the softmax warps write the results before.
+            if (ok && elect_one()) {
+              mbar_expect(q_full + x, (DP / 64) * 128u * P.group * P.tile_tokens);
+#pragma unroll
+              for (int d = 0; d < DP / 64; ++d)
+                tma_load_3d(base + x * Z::kTile + d * kHalf, &QM, 64 * d, p.h * P.group, p.s.row0 + p.t0 + x * P.tile_tokens, smem_addr(q_full + x));
+            }
+            __syncwarp();
+            wait(q_full + x, q_count++ & 1);
+          }
           wait(full + k_stage, k_ph);
-          if (first) wait(q_full + x, q_count++ & 1);
-          else weighted_sum(j == r.first + 1);
+          if (!first) weighted_sum(j == r.first + 1);
           if (!ok) break;
           any = true;
           const uint64_t k = smem_desc_sw128(ring + k_stage * Z::kTile);
