@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   constexpr int kStages = Z::kStages;
   constexpr uint32_t kHalf = 128 * 128;   // bytes of 64 columns of a tile: 128 rows of 128 bytes, swizzled
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[2], s_full[2], p_full[2], o_full[2], mma_done[2], tail_full;
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], mma_done[2], tail_full;
   __shared__ uint32_t tmem_slot[1];
   __shared__ int abort_word, s_first[4];
   __shared__ long long s_scan[kPromptThreads / 32], s_rest;
@@ -262,6 +262,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(smem_addr(q_full + x), 1);
+      mbar_init(smem_addr(q_empty + x), 4);
       mbar_init(smem_addr(s_full + x), 1);
       mbar_init(smem_addr(p_full + x), 4);
       mbar_init(smem_addr(o_full + x), 1);
@@ -369,6 +370,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // a scale of 0 becomes a very small one: a score hidden as -inf must stay -inf
     const float c = fmaxf(fabsf(P.a.scale) * 1.4426950408889634f, 1e-30f);
     const bool leader = (warp & 3) == 0 && lane == 0;
+    uint8_t* const mine_rows = smem_raw + x * Z::kTile + (warp & 3) * (Z::kTile / 4);   // 32 rows of the queries' place
     int s_count = 0, o_count = 0, stage = 0, v_before = 0;
     auto mend_rows = [&](const Piece& p, const TileRange& r, bool bad, int pos, int lo, int head, int token) {
       uint32_t rows = __ballot_sync(0xffffffffu, bad);
@@ -472,41 +474,62 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (leader && !r.none()) mbar_arrive(empty + v_before);
       float check = 0.f;
       if (!idle) {
-        const bool whole = p.begins && p.ends, empty = pos < 0 || r.none();
+        const bool whole = p.begins && p.ends && !r.none(), empty = pos < 0;
         const float f = empty ? 0.f : 1.f / l;
-        T* out = static_cast<T*>(P.a.out) + static_cast<long long>(p.s.row0 + p.t0 + x * P.tile_tokens + token) * P.a.out_token +
-                 static_cast<long long>(p.h * P.group + head) * P.a.out_head;
         float* part = P.partial + (static_cast<size_t>(blockIdx.x) * 4 + (p.begins ? 2 : 0) + x) * tile_partial_floats(P.dim16);
-        if (!whole) {
+        if (!(p.begins && p.ends)) {
           part[row] = pos < 0 ? -INFINITY : m;
           part[128 + row] = pos < 0 ? 0.f : l;
         }
 #pragma unroll 1
-        for (int d0 = 0; d0 < P.dim16; d0 += 32) {
+        for (int d0 = 0; d0 < P.dim16 && !r.none(); d0 += 32) {
           uint32_t o[32];
-          if (!r.none()) {
-            tmem_load16_at(to + d0, o);
-            if (d0 + 16 < P.dim16) tmem_load16_at(to + d0 + 16, o + 16);
-            tmem_wait_load();
-          }
+          tmem_load16_at(to + d0, o);
+          if (d0 + 16 < P.dim16) tmem_load16_at(to + d0 + 16, o + 16);
+          tmem_wait_load();
           if (whole) {
 #pragma unroll
             for (int d = 0; d < 32; d += 8) {
               uint32_t h[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k) h[k] = empty ? 0u : pack2<T>(__uint_as_float(o[d + 2 * k]) * f, __uint_as_float(o[d + 2 * k + 1]) * f);
-              if (mine && d0 + d < P.a.pool.Dh) {
-                *reinterpret_cast<uint4*>(out + d0 + d) = make_uint4(h[0], h[1], h[2], h[3]);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) check = fmaf(__uint_as_float(o[d + k]), 0.f, check);   // NaN from the first that is not finite on
-              }
+              for (int k = 0; k < 8; ++k) check = d0 + d < P.a.pool.Dh ? fmaf(__uint_as_float(o[d + k]), 0.f, check) : check;   // NaN from the first that is not finite on
+              if (d0 + d < DP) *reinterpret_cast<uint4*>(mine_rows + lane * (DP * 2) + ((((d0 + d) >> 3) ^ (lane & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
             }
-          } else if (!r.none()) {
+          } else {
 #pragma unroll
             for (int d = 0; d < 32; d += 4)
               if (d0 + d < P.dim16) *reinterpret_cast<uint4*>(part + 256 + (static_cast<size_t>((d0 + d) / 4) * 128 + row) * 4) = make_uint4(o[d], o[d + 1], o[d + 2], o[d + 3]);
           }
         }
+      }
+      if (r.none() && p.begins && p.ends) {   // rows that see nothing
+        if (mine)
+          for (int d = 0; d < P.a.pool.Dh; d += 8)
+            *reinterpret_cast<uint4*>(static_cast<T*>(P.a.out) + static_cast<long long>(p.s.row0 + p.t0 + x * P.tile_tokens + token) * P.a.out_token +
+                                      static_cast<long long>(p.h * P.group + head) * P.a.out_head + d) = make_uint4(0u, 0u, 0u, 0u);
+      } else if (!idle && p.begins && p.ends) {
+        // Row by row through the place of this tile's queries: a warp's store covers whole rows, not 16 bytes of 32 rows each, which
+        // kept the load/store unit busy for 4000 cycles per pair.
+        const uint32_t rows = __ballot_sync(0xffffffffu, mine);
+        const unsigned long long my_out = reinterpret_cast<unsigned long long>(static_cast<T*>(P.a.out) + static_cast<long long>(p.s.row0 + p.t0 + x * P.tile_tokens + token) * P.a.out_token +
+                                                                              static_cast<long long>(p.h * P.group + head) * P.a.out_head);
+        __syncwarp();
+        constexpr int kChunks = DP / 8, kRowsAtOnce = 32 / kChunks;
+        const int chunk = lane % kChunks;
+#pragma unroll 4
+        for (int i = 0; i < kChunks; ++i) {
+          const int src = i * kRowsAtOnce + lane / kChunks;
+          const unsigned long long to_row = __shfl_sync(0xffffffffu, my_out, src);
+          const uint4 v = *reinterpret_cast<const uint4*>(mine_rows + src * (DP * 2) + ((chunk ^ (src & 7)) << 4));
+          if ((rows >> src & 1u) && chunk * 8 < P.a.pool.Dh) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(to_row) + chunk * 8) = v;
+        }
+      }
+      if (!r.none()) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next queries come here
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_empty + x);
       }
       if (!idle && p.begins && p.ends) mend_rows(p, r, check != 0.f && pos >= 0 && !r.none() && !not_finite(l), pos, lo, head, token);
       tc_fence_before();   // the next P is announced after these reads of O
@@ -631,8 +654,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
           const bool first = j == r.first, last = j + 1 == r.last;
           if (first) {
-            // This tile's queries.  The multiplications that read the last ones are done: their scores have become the P of the last
-            // weighted sum.  The latency passes while the softmax warps write the results before.
+            // This tile's queries, once the results before have left through their place.  (The multiplications that read the last
+            // ones are done: their scores have become the P of the last weighted sum.)
+            wait(q_empty + x, (q_count & 1) ^ 1);
             if (ok && elect_one()) {
               mbar_expect(q_full + x, (DP / 64) * 128u * P.group * P.tile_tokens);
 #pragma unroll
