@@ -329,7 +329,8 @@ int lw_cache_append(void* cache, const void* qkv, int qkv_type, long long row_st
 long long lw_cache_workspace(void* cache, int n_heads, int prompt);
 
 /* Attention of one new token per sequence: out[b][h] = sum_j softmax_j(scale q[b][h] . k_j) v_j over the positions
- * max(0, lens[b] - window) <= j < lens[b] (window 0: from 0).  Query head h reads kv head h / (n_heads / n_kv_heads).  q and out in
+ * max(0, lens[b] - window) <= j < lens[b] (window 0: from 0).  Query head h reads kv head h / (n_heads / n_kv_heads), at most 128
+ * query heads per kv head.  q and out in
  * the cache's type, rows and heads on 16-byte boundaries.  A sequence of length 0 gives zeros. */
 int lw_cache_attend(void* cache, const void* q, long long q_token_stride, long long q_head_stride, int n_seqs, int n_heads, const int* lens,
                     const int* table, int table_cols, long long table_stride, float scale, int window, void* out,
@@ -362,8 +363,8 @@ long long lw_launch_count(void);
 /* Test switches (no reference counterpart).  Keys: "max_units" (2..1024: units a block is dealt per launch; smaller
  * values make a product run as several launches over ranges of tile rows, the path very tall matrices take),
  * "wait_limit" (polls after which a device-side wait gives up), "drop_unit" (block 0 of the one-row kernel never copies this unit
- * of its list, block 0 of the GEMM over decoded weights this 64-column slab of its first tile, so the waits for it run
- * out; -1 = none), "t5_min_rows" (1..65: products of at least this many rows,
+ * of its list, block 0 of the GEMM over decoded weights this 64-column slab of its first tile, the first warp or block of the paged attention this
+ * load of its share, so the waits for it run out; -1 = none), "t5_min_rows" (1..65: products of at least this many rows,
  * and at most 64, take the decode + tcgen05 kernel; 9 in production), "pairs" (0 / 1: product kernels read the bundle's own code even
  * where a matrix has a pair layout), "attn_rows" (0: passes of several tokens take the attention kernel with a block per token, not
  * the tiled one; passes captured before keep theirs), "reset" (all back to the production values). */

@@ -10,13 +10,21 @@
 //  P            one thread per row reads S, writes P in the cache's type over S
 //  O += P V     tcgen05.mma, P from tensor memory, V from shared memory as it lies in the pages (positions are its K axis)
 //
-// Bound: the tensor core and the exponentials, about even: a block of 128 x 128 x 128 is 1024 cycles of each per SM.  So two
-// tiles of 128 rows (a pair) share the staged keys and values of a thread block and take turns: while one tile's softmax runs
-// the tensor core works for the other.
-//  * Warp 0 loads (TMA; a page's rows of a kv head are a box), warp 1 issues the multiplications, warps 4..7 and 8..11 are the
-//    softmax of the two tiles.  K and V blocks go through one ring of stages.
-//  * The work is cut into equal shares whatever the lengths (lw_attend_plan.h); a pair that is cut leaves unnormalised partial
-//    results, which k_attend_join adds up.  Lengths are read on the device.
+// Bound: the tensor core and the exponentials, about even: 128 x 128 x 128 take 1067 cycles of multiplications (554 + 513, measured) and
+// 1024 of exponentials (16 per cycle and SM).  So two tiles of 128 rows (a pair) share the staged keys and values of a thread block and
+// take turns: while one tile's softmax runs the tensor core works for the other.  What a block of positions takes now, 3350
+// cycles for both tiles, is the chain of one tile: 2000 cycles of softmax (scores in 450, exponentials 1400: the special-function
+// unit serves both tiles), then its multiplications and two hand-overs.  16384 tokens, 32 heads over 8: 1.98 ms, 1110
+// TFLOP/s of what the mask leaves; 509 tokens behind 32000: 252 us, 1070.
+//  * Warp 0 loads keys and warp 2 values (TMA; a page's rows of a kv head are a box) into one ring of stages.  Warps 1 and 3 issue the
+//    multiplications of a tile each, and load its queries: issuing blocks while the tensor core is busy, and a commit costs it 78
+//    cycles, so one warp for both tiles with commits for the stages left it idle a third more.  Warps 4..7 and 8..11 are the softmax
+//    of the two tiles; they tell when a stage is read, from the completion of the scores behind it.
+//  * A thread holds a whole row of S, 128 registers: with two threads per row the exponentials took as long (the special-function unit) and
+//    the maximum had to be exchanged.  A third of the exponentials as polynomials on the other pipes changed nothing: the warps are
+//    bound by what they issue.  P handed over in halves made the exponentials slower than it made the product earlier.
+//  * The work is cut into equal shares whatever the lengths (lw_attend_plan.h), a pair's start and end counted as kPromptLead blocks
+//    of positions; a pair that is cut leaves unnormalised partial results, which k_attend_join adds up.  Lengths are read on the device.
 //  * Values of positions that no row of the pair sees are zeroed in shared memory before they are multiplied (a weight of 0
 //    would not hide a NaN that an earlier owner of the page left).
 //  * Rounding: S, m, l, O in 32 bits; P in the cache's type, as the tensor core takes it (half a step of its 11 or 8 bits,
@@ -33,12 +41,12 @@ namespace lw {
 
 constexpr int kPromptThreads = 12 * 32;
 constexpr int kPromptRegsSoftmax = 216, kPromptRegsOther = 72;   // 8 and 4 warps: 12 x 168, the launch's
-constexpr float kSlack = 8.f;
-constexpr int kPromptLead = 3;
+constexpr float kSlack = 8.f;         // of a row's maximum, in powers of two, before its reference follows
+constexpr int kPromptLead = 3;       // 24 packed prompts of 20 to 2500 tokens: 248 us (0: 411, 1: 283, 2: 244); 16384 tokens: 1.98 ms (1: 2.10, 2: 2.02)
 
 // The pair that block c continues: its first packed row, rows (tokens) and first query head, and the blocks that hold its first and
 // last unit (first == c: none).  A block leaves the pair that it continues as its piece 0, the one that it only begins as piece 1.
-struct PieceNote {
+struct alignas(16) PieceNote {
   int row0, rows, head0, first, last;
   int b, position, pad;   // its sequence, position of its first token
 };
@@ -721,7 +729,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
   pdl_trigger();
   pdl_wait();
   const int c = blockIdx.x + 1, x = blockIdx.y >> 2, row = (blockIdx.y & 3) * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
-  const PieceNote n = P.notes[c];
+  // what the kernel before wrote is read from L2
+  const int4 note_a = __ldcg(reinterpret_cast<const int4*>(P.notes + c)), note_b = __ldcg(reinterpret_cast<const int4*>(P.notes + c) + 1);
+  const PieceNote n = {note_a.x, note_a.y, note_a.z, note_a.w, note_b.x, note_b.y, note_b.z, 0};
   if (n.first != c - 1) return;   // nothing continued, or not the first to continue it
   const int token = row / P.group, head = row - token * P.group, t = x * P.tile_tokens + token;
   const bool mine = token < P.tile_tokens && t < n.rows;
@@ -730,7 +740,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
   auto piece = [&](int k) { return P.partial + (static_cast<size_t>(k) * 4 + (k < c ? 2 : 0) + x) * tile; };
   float m = -INFINITY, l = 0.f;
 #pragma unroll 4
-  for (int k = c - 1; k <= last; ++k) m = fmaxf(m, piece(k)[row]);
+  for (int k = c - 1; k <= last; ++k) m = fmaxf(m, __ldcg(piece(k) + row));
   const float ref = m == -INFINITY ? 0.f : m;
   constexpr int kWarps = kJoinThreads / 32, kSteps = 128 / (4 * kWarps);
   float4 o[kSteps];
@@ -738,14 +748,14 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
   for (int i = 0; i < kSteps; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k = c - 1; k <= last; ++k) {
     const float* part = piece(k);
-    const float lk = part[128 + row], f = exp2_fast(part[row] - ref);
+    const float lk = __ldcg(part + 128 + row), f = exp2_fast(__ldcg(part + row) - ref);
     l += lk * f;
     if (lk == 0.f) continue;   // the piece holds nothing for this row, and no O
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       const int d = (i * kWarps + warp) * 4;
       if (d < P.dim16) {
-        const float4 v = *reinterpret_cast<const float4*>(part + 256 + (static_cast<size_t>(d / 4) * 128 + row) * 4);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(part + 256 + (static_cast<size_t>(d / 4) * 128 + row) * 4));
         o[i] = make_float4(fmaf(f, v.x, o[i].x), fmaf(f, v.y, o[i].y), fmaf(f, v.z, o[i].z), fmaf(f, v.w, o[i].w));
       }
     }

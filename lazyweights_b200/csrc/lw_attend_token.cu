@@ -36,7 +36,7 @@ constexpr int kTokenBlocksPerSm = 2;
 constexpr int kLead = 2;                  // see above: 200 sequences of 10 to 500 positions, 8 kv heads: 32.1 us (0: 41.7, 1: 34.5, 4: 32.5)
 
 // The piece that worker w continues: sequence, head slot, the workers that hold its first and last unit (first == w: none).
-struct TokenNote {
+struct alignas(16) TokenNote {
   int b, h, first, last;
 };
 
@@ -455,6 +455,11 @@ __global__ void __launch_bounds__(kTokenJoinThreads) k_token_join(const __grid_c
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, all = (workers - 1) * kJobs;
+  // what the kernel before wrote is read from L2
+  auto note_of = [&](int w) {
+    const int4 v = __ldcg(reinterpret_cast<const int4*>(P.notes + w));
+    return TokenNote{v.x, v.y, v.z, v.w};
+  };
   auto piece_of = [&](const TokenNote& n, int k) { return P.partial + (static_cast<size_t>(k) * 2 + (k == n.first ? 1 : 0)) * Z::kPartial; };
   auto result = [&](const TokenNote& n, int nt, int step, const float4& sum, const float* total) {
     const float f[2] = {1.f / total[0], 1.f / total[1]};
@@ -464,13 +469,13 @@ __global__ void __launch_bounds__(kTokenJoinThreads) k_token_join(const __grid_c
   };
   constexpr int kGroup = Z::kSteps < 4 ? Z::kSteps : 4, kGroups = kJobs / kGroup;   // steps of a short job
   for (int j = blockIdx.x + warp * gridDim.x; j < (workers - 1) * kGroups; j += gridDim.x * kTokenJoinWarps) {
-    const TokenNote n = P.notes[j / kGroups + 1];
+    const TokenNote n = note_of(j / kGroups + 1);
     if (n.first != j / kGroups || n.last - n.first >= kTokenShort) continue;
     const int first_job = j % kGroups * kGroup, nt = first_job / Z::kSteps;
     float4 ml[kTokenShort];
 #pragma unroll
     for (int q = 0; q < kTokenShort; ++q)
-      ml[q] = n.first + q <= n.last ? *reinterpret_cast<const float4*>(piece_of(n, n.first + q) + (nt * 8 + (lane & 3) * 2) * 2) : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+      ml[q] = n.first + q <= n.last ? __ldcg(reinterpret_cast<const float4*>(piece_of(n, n.first + q) + (nt * 8 + (lane & 3) * 2) * 2)) : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     float4 o[kGroup];
 #pragma unroll
@@ -489,7 +494,7 @@ __global__ void __launch_bounds__(kTokenJoinThreads) k_token_join(const __grid_c
       for (int q = 0; q < 4; ++q)
 #pragma unroll
         for (int k = 0; k < kGroup; ++k)
-          v[q][k] = n.first + q0 + q <= n.last ? *reinterpret_cast<const float4*>(piece_of(n, n.first + q0 + q) + Z::kPartHead + ((first_job + k) * 32 + lane) * 4)
+          v[q][k] = n.first + q0 + q <= n.last ? __ldcg(reinterpret_cast<const float4*>(piece_of(n, n.first + q0 + q) + Z::kPartHead + ((first_job + k) * 32 + lane) * 4))
                                                : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -510,7 +515,7 @@ __global__ void __launch_bounds__(kTokenJoinThreads) k_token_join(const __grid_c
     const int j = j0 + tid * gridDim.x + blockIdx.x;
     if (j < all) {
       const int w = j / kJobs + 1;
-      const TokenNote n = P.notes[w];
+      const TokenNote n = note_of(w);
       if (n.first == w - 1 && n.last - n.first >= kTokenShort) {
         const int at = atomicAdd(&s_jobs, 1);
         s_job[at] = j % kJobs;
@@ -527,8 +532,8 @@ __global__ void __launch_bounds__(kTokenJoinThreads) k_token_join(const __grid_c
 #pragma unroll 4
       for (int k = n.first + warp; k <= n.last; k += kTokenJoinWarps) {
         const float* p = piece_of(n, k);
-        const float4 ml = *reinterpret_cast<const float4*>(p + (nt * 8 + (lane & 3) * 2) * 2);   // (m, l) of the lane's two heads
-        const float4 v = *reinterpret_cast<const float4*>(p + Z::kPartHead + (job * 32 + lane) * 4);
+        const float4 ml = __ldcg(reinterpret_cast<const float4*>(p + (nt * 8 + (lane & 3) * 2) * 2));   // (m, l) of the lane's two heads
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p + Z::kPartHead + (job * 32 + lane) * 4));
         const float mk[2] = {ml.x, ml.z}, lk[2] = {ml.y, ml.w};
         float keep[2], add[2];
 #pragma unroll
