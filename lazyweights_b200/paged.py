@@ -31,7 +31,7 @@ class PagedCache:
 
     def __init__(self, k_pages, v_pages):
         torch = _torch()
-        self._h, self._spaces = None, {}
+        self._h, self._spaces, self._lib = None, {}, nat.lib()
         if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype is not v_pages.dtype or \
                 k_pages.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError("PagedCache wants two fp16 or bf16 pools [pages, kv_heads, page_size, head_dim] of one shape and type")
@@ -45,9 +45,9 @@ class PagedCache:
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = n, heads, size, dim
         self.dtype, self.device, self._index = k_pages.dtype, k_pages.device, k_pages.get_device()
         with torch.cuda.device(self._index):
-            ptr = nat.lib().lw_cache_create(k_pages.data_ptr(), v_pages.data_ptr(), _codes(torch)[self.dtype], n, heads, size, dim, sp, sh, st)
+            ptr = self._lib.lw_cache_create(k_pages.data_ptr(), v_pages.data_ptr(), _codes(torch)[self.dtype], n, heads, size, dim, sp, sh, st)
         if not ptr:
-            raise nat.LwError(nat.lib().lw_last_status() or -1, nat.last_error())
+            raise nat.LwError(self._lib.lw_last_status() or -1, nat.last_error())
         self._h = ptr
 
     @classmethod
@@ -60,7 +60,7 @@ class PagedCache:
 
     def close(self):
         if self._h:
-            nat.lib().lw_cache_destroy(self._h)
+            self._lib.lw_cache_destroy(self._h)
             self._h = None
 
     def __del__(self):
@@ -69,16 +69,18 @@ class PagedCache:
         except Exception:
             pass
 
-    # ---- checks
+    # ---- checks.  A call on a few rows takes the GPU 2 to 20 us, so what the checks cost counts: one call per property.
     def _sequences(self, torch, table, lens):
         i32 = torch.int32
-        if table.dtype is not i32 or lens.dtype is not i32 or table.dim() != 2 or lens.dim() != 1 or table.shape[0] != lens.shape[0] or \
+        n = lens.shape[0] if lens.dim() == 1 else -1
+        if table.dtype is not i32 or lens.dtype is not i32 or table.dim() != 2 or table.shape[0] != n or \
                 table.get_device() != self._index or lens.get_device() != self._index:
             raise ValueError("table [n, columns] and lens [n] must be int32 on the cache's device")
-        n, cols = table.shape
-        if cols > 1 and table.stride(1) != 1 or n > 1 and lens.stride(0) != 1:
+        cols = table.shape[1]
+        st, sc = table.stride()
+        if cols > 1 and sc != 1 or n > 1 and lens.stride(0) != 1:
             raise ValueError("the rows of table, and lens, must be contiguous")
-        return n, cols, table.stride(0) if n > 1 else max(cols, 1)
+        return n, cols, st if n > 1 else max(cols, 1)
 
     def _starts(self, torch, starts, n):
         if starts.dtype is not torch.int32 or starts.dim() != 1 or starts.shape[0] != n + 1 or starts.get_device() != self._index or \
@@ -86,13 +88,16 @@ class PagedCache:
             raise ValueError("starts [%d] must be contiguous int32 on the cache's device" % (n + 1))
 
     def _rows(self, t, what, rows=None, heads=None):
-        """Strides of a [rows, heads, head_dim] tensor of queries or results."""
-        if t.dim() != 3 or t.dtype is not self.dtype or t.get_device() != self._index or t.shape[2] != self.head_dim or t.stride(2) != 1 or \
-                (rows is not None and (t.shape[0] != rows or t.shape[1] != heads)):
-            raise ValueError("%s must be [rows, heads, %d] of the cache's type and device, head_dim contiguous" % (what, self.head_dim))
-        r, h = t.shape[0], t.shape[1]
-        sh = t.stride(1) if h > 1 else self.head_dim
-        return (t.stride(0) if r > 1 else h * sh), sh
+        """Rows, heads and strides of a [rows, heads, head_dim] tensor of queries or results."""
+        if t.dim() == 3 and t.dtype is self.dtype and t.get_device() == self._index:
+            r, h, d = t.shape
+            sr, sh, sd = t.stride()
+            if d == self.head_dim and sd == 1 and (rows is None or r == rows) and (heads is None or h == heads):
+                if h == 1:
+                    sh = d
+                return r, h, (sr if r > 1 else h * sh), sh
+        raise ValueError("%s must be [%s, %s, %d] of the cache's type and device, head_dim contiguous"
+                         % (what, "rows" if rows is None else rows, "heads" if heads is None else heads, self.head_dim))
 
     # ---- operators
     def append(self, qkv, n_heads, cos, sin, table, lens, starts=None, q=None):
@@ -101,25 +106,25 @@ class PagedCache:
         tables [positions, r], pairs (i, i + r) are rotated, dimensions from 2 r on copied.  Without starts, row b is the last position
         of sequence b.  Rows of no sequence are left as they are, in q too."""
         torch = _torch()
+        index = self._index
         n, cols, tstride = self._sequences(torch, table, lens)
         if starts is not None:
             self._starts(torch, starts, n)
-        code = _codes(torch).get(qkv.dtype)
-        if qkv.dim() != 2 or code is None or qkv.get_device() != self._index or qkv.shape[1] != (n_heads + 2 * self.kv_heads) * self.head_dim or \
-                qkv.stride(1) != 1:
-            raise ValueError("qkv must be [rows, %d] fp16, bf16 or fp32 on the cache's device" % ((n_heads + 2 * self.kv_heads) * self.head_dim))
+        code, width = _codes(torch).get(qkv.dtype), (n_heads + 2 * self.kv_heads) * self.head_dim
+        if qkv.dim() != 2 or code is None or qkv.get_device() != index or qkv.shape[1] != width or qkv.stride(1) != 1:
+            raise ValueError("qkv must be [rows, %d] fp16, bf16 or fp32 on the cache's device" % width)
         f32 = torch.float32
         if cos.dtype is not f32 or sin.dtype is not f32 or cos.dim() != 2 or cos.shape != sin.shape or not cos.is_contiguous() or \
-                not sin.is_contiguous() or cos.get_device() != self._index or sin.get_device() != self._index:
+                not sin.is_contiguous() or cos.get_device() != index or sin.get_device() != index:
             raise ValueError("cos and sin must be contiguous fp32 tables [positions, pairs] on the cache's device")
         rows = qkv.shape[0]
         if q is None:
             q = torch.empty((rows, n_heads, self.head_dim), dtype=self.dtype, device=self.device)
-        qt, qh = self._rows(q, "q", rows, n_heads)
-        rc = nat.lib().lw_cache_append(self._h, qkv.data_ptr(), code, qkv.stride(0) if rows > 1 else qkv.shape[1], rows, n_heads,
-                                       cos.data_ptr(), sin.data_ptr(), cos.shape[0], cos.shape[1],
-                                       None if starts is None else starts.data_ptr(), lens.data_ptr(), table.data_ptr(), n, cols, tstride,
-                                       q.data_ptr(), qt, qh, _stream(torch, self._index))
+        _, _, qt, qh = self._rows(q, "q", rows, n_heads)
+        positions, pairs = cos.shape
+        rc = self._lib.lw_cache_append(self._h, qkv.data_ptr(), code, qkv.stride(0) if rows > 1 else width, rows, n_heads, cos.data_ptr(),
+                                       sin.data_ptr(), positions, pairs, None if starts is None else starts.data_ptr(), lens.data_ptr(),
+                                       table.data_ptr(), n, cols, tstride, q.data_ptr(), qt, qh, _stream(torch, index))
         if rc < 0:
             nat.check(rc)
         return q
@@ -128,7 +133,7 @@ class PagedCache:
         """A workspace of the call's own: calls may overlap, and captured ones too."""
         need = self._spaces.get((heads, prompt))
         if need is None:
-            need = self._spaces[heads, prompt] = nat.check(nat.lib().lw_cache_workspace(self._h, heads, prompt))
+            need = self._spaces[heads, prompt] = nat.check(self._lib.lw_cache_workspace(self._h, heads, prompt))
         return torch.empty(need, dtype=torch.uint8, device=self.device), need
 
     def attend(self, q, table, lens, scale=None, window=0, out=None):
@@ -137,14 +142,14 @@ class PagedCache:
         gives zeros."""
         torch = _torch()
         n, cols, tstride = self._sequences(torch, table, lens)
-        qt, qh = self._rows(q, "q", n, q.shape[1])
+        _, heads, qt, qh = self._rows(q, "q", n)
         if out is None:
-            out = torch.empty((n, q.shape[1], self.head_dim), dtype=self.dtype, device=self.device)
-        ot, oh = self._rows(out, "out", n, q.shape[1])
-        space, size = self._workspace(torch, q.shape[1], 0)
-        rc = nat.lib().lw_cache_attend(self._h, q.data_ptr(), qt, qh, n, q.shape[1], lens.data_ptr(), table.data_ptr(), cols, tstride,
-                                       self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(), ot, oh,
-                                       space.data_ptr(), size, _stream(torch, self._index))
+            out = torch.empty((n, heads, self.head_dim), dtype=self.dtype, device=self.device)
+        _, _, ot, oh = self._rows(out, "out", n, heads)
+        space, size = self._workspace(torch, heads, 0)
+        rc = self._lib.lw_cache_attend(self._h, q.data_ptr(), qt, qh, n, heads, lens.data_ptr(), table.data_ptr(), cols, tstride,
+                                       self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(), ot, oh, space.data_ptr(), size,
+                                       _stream(torch, self._index))
         if rc < 0:
             nat.check(rc)
         return out
@@ -156,15 +161,14 @@ class PagedCache:
         torch = _torch()
         n, cols, tstride = self._sequences(torch, table, lens)
         self._starts(torch, starts, n)
-        qt, qh = self._rows(q, "q")
-        rows, heads = q.shape[0], q.shape[1]
+        rows, heads, qt, qh = self._rows(q, "q")
         if out is None:
             out = torch.empty((rows, heads, self.head_dim), dtype=self.dtype, device=self.device)
-        ot, oh = self._rows(out, "out", rows, heads)
+        _, _, ot, oh = self._rows(out, "out", rows, heads)
         space, size = self._workspace(torch, heads, 1)
-        rc = nat.lib().lw_cache_attend_prompt(self._h, q.data_ptr(), qt, qh, rows, heads, starts.data_ptr(), lens.data_ptr(), table.data_ptr(),
-                                              n, cols, tstride, self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
-                                              ot, oh, space.data_ptr(), size, _stream(torch, self._index))
+        rc = self._lib.lw_cache_attend_prompt(self._h, q.data_ptr(), qt, qh, rows, heads, starts.data_ptr(), lens.data_ptr(), table.data_ptr(), n, cols,
+                                              tstride, self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(), ot, oh,
+                                              space.data_ptr(), size, _stream(torch, self._index))
         if rc < 0:
             nat.check(rc)
         return out
