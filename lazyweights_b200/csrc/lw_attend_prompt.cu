@@ -429,10 +429,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           tmem_load32(ts + 96, v + 96);
           tmem_wait_load();
           if (__builtin_expect(p0 + kPosBlock - 1 > r.p_first || (P.a.window > 0 && p0 <= r.p_last - P.a.window), 0)) {   // some row does not see all of it
-            const int top = pos - p0, bottom = lo - p0;
+            // which columns, as bits: one selection per score (two comparisons more, and their code, took as long as the exponentials)
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (i > top || i < bottom) v[i] = 0xff800000u;
+            for (int k = 0; k < 4; ++k) {
+              const int top = pos - p0 - 32 * k, bottom = lo - p0 - 32 * k;
+              uint32_t seen = top >= 31 ? 0xffffffffu : top < 0 ? 0u : (2u << top) - 1u;
+              seen &= bottom <= 0 ? 0xffffffffu : bottom >= 32 ? 0u : 0xffffffffu << bottom;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(seen >> i & 1u)) v[32 * k + i] = 0xff800000u;
+            }
           }
 #pragma unroll
           for (int i = 0; i < 128; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
@@ -593,9 +599,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (cut) {
             ok = wait_warp(&tail_full, tails++ & 1, P.wait_limit, P.a.err, abort_flag);
             uint8_t* dst = smem_raw + (stage - smem_addr(smem_raw));
-            for (int n = lane; n < kPosBlock * kHalves * 8; n += 32) {
-              const int row = (n >> 3) & 127, half = n >> 10;
-              if (row >= end || row < begin) *reinterpret_cast<uint4*>(dst + half * kHalf + row * 128 + (n & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            for (int n = lane; n < (kPosBlock - end + begin) * 8; n += 32) {   // rows end .. 127, then 0 .. begin - 1
+              const int row = (end + (n >> 3)) & (kPosBlock - 1);
+#pragma unroll
+              for (int d = 0; d < kHalves; ++d) *reinterpret_cast<uint4*>(dst + d * kHalf + row * 128 + (n & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
