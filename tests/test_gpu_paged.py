@@ -234,6 +234,57 @@ def test_strided_queries_and_results(lw):
 
 
 @pytest.mark.parametrize("prompt", [True, False])
+def test_heads_outside_the_rows(lw, prompt):
+    """Queries and results [heads][rows][dim], passed transposed; pools with the heads outermost."""
+    import torch
+    pr = problem([300, 41], [70, 41] if prompt else [1, 1], 6, 3, 96, 16, "fp16", seed=8)
+    rows = pr["q"].shape[0]
+    turned = [pr[n].cuda().transpose(0, 1).contiguous().transpose(0, 1) for n in ("k", "v")]
+    cache = lw.PagedCache(*turned)
+    q = pr["q"].cuda().transpose(0, 1).contiguous().transpose(0, 1)
+    assert q.stride(1) == rows * 96 and turned[0].stride(1) > turned[0].stride(0)
+    out = torch.full((6, rows, 96), 7.0, dtype=torch.float16, device="cuda").transpose(0, 1)
+    args = [pr[n].cuda() for n in ("table", "lens")] + ([pr["starts"].cuda()] if prompt else [])
+    (cache.attend_prompt if prompt else cache.attend)(q, *args, out=out)
+    plain = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+    assert torch.equal(out, (plain.attend_prompt if prompt else plain.attend)(pr["q"].cuda(), *args))
+    check_attention(lw, pr, prompt=prompt)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(128, 1), (100, 1), (129 * 2 - 2, 2)])
+def test_wide_groups(lw, heads, kv_heads):
+    """Up to 128 query heads per kv head: one token per tile of rows."""
+    for prompt in (True, False):
+        check_attention(lw, problem([150, 3], [9, 3] if prompt else [1, 1], heads, kv_heads, 64, 16, "fp16", seed=heads), prompt=prompt)
+
+
+def test_one_large_page(lw):
+    for prompt in (True, False):
+        check_attention(lw, problem([1000], [200 if prompt else 1], 4, 2, 64, 4096, "bf16", seed=1), prompt=prompt)
+
+
+def test_thousands_of_sequences(lw):
+    """More sequences than a block has threads, several times over, most of them short or without rows."""
+    import torch
+    lens = [(i * 7) % 23 for i in range(3000)]
+    check_attention(lw, problem(lens, [1] * 3000, 2, 1, 32, 8, "fp16", seed=2), prompt=False)
+    news = [min(n, i % 3) for i, n in enumerate(lens)]
+    check_attention(lw, problem(lens, news, 2, 1, 32, 8, "fp16", seed=3, gap=2))
+
+
+def test_rows_before_the_first_sequence(lw):
+    import torch
+    pr = problem([50, 20], [5, 20], 4, 2, 64, 16, "fp16")
+    cache = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+    table, lens = pr["table"].cuda(), pr["lens"].cuda()
+    want = cache.attend_prompt(pr["q"].cuda(), table, lens, pr["starts"].cuda())
+    q = torch.cat((torch.zeros(3, 4, 64, dtype=torch.float16), pr["q"])).cuda()
+    out = torch.full_like(q, 7.0)
+    cache.attend_prompt(q, table, lens, (pr["starts"] + 3).cuda(), out=out)
+    assert (out[:3] == 7).all() and torch.equal(out[3:], want)
+
+
+@pytest.mark.parametrize("prompt", [True, False])
 def test_same_call_same_bits(lw, prompt):
     import torch
     pr = problem([3000, 17], [200, 17] if prompt else [1, 1], 8, 2, 128, 16, "fp16")
