@@ -14,8 +14,8 @@
 // 1024 of exponentials (16 per cycle and SM).  So two tiles of 128 rows (a pair) share the staged keys and values of a thread block and
 // take turns: while one tile's softmax runs the tensor core works for the other.  What a block of positions takes now, 3350
 // cycles for both tiles, is the chain of one tile: 2000 cycles of softmax (scores in 450, exponentials 1400: the special-function
-// unit serves both tiles), then its multiplications and two hand-overs.  16384 tokens, 32 heads over 8: 1.98 ms, 1110
-// TFLOP/s of what the mask leaves; 509 tokens behind 32000: 252 us, 1070.
+// unit serves both tiles), then its multiplications and two hand-overs.  16384 tokens, 32 heads over 8: 2.0 to 2.2 ms with
+// the card's clock under its power limit, 1000 to 1100 TFLOP/s of what the mask leaves; 509 tokens behind 32000: 253 us, 1065.
 //  * Warp 0 loads keys and warp 2 values (TMA; a page's rows of a kv head are a box) into one ring of stages.  Warps 1 and 3 issue the
 //    multiplications of a tile each, and load its queries: issuing blocks while the tensor core is busy, and a commit costs it 78
 //    cycles, so one warp for both tiles with commits for the stages left it idle a third more.  Warps 4..7 and 8..11 are the softmax
@@ -42,7 +42,7 @@ namespace lw {
 constexpr int kPromptThreads = 12 * 32;
 constexpr int kPromptRegsSoftmax = 216, kPromptRegsOther = 72;   // 8 and 4 warps: 12 x 168, the launch's
 constexpr float kSlack = 8.f;         // of a row's maximum, in powers of two, before its reference follows
-constexpr int kPromptLead = 3;       // 24 packed prompts of 20 to 2500 tokens: 248 us (0: 411, 1: 283, 2: 244); 16384 tokens: 1.98 ms (1: 2.10, 2: 2.02)
+constexpr int kPromptLead = 2;       // 24 packed prompts of 20 to 2500 tokens: 234 us (0: 362, 1: 265, 3: 237)
 
 // The pair that block c continues: its first packed row, rows (tokens) and first query head, and the blocks that hold its first and
 // last unit (first == c: none).  A block leaves the pair that it continues as its piece 0, the one that it only begins as piece 1.
