@@ -16,7 +16,8 @@
 // cycles for both tiles, is the chain of one tile: 2000 cycles of softmax (scores in 450, exponentials 1400: the special-function
 // unit serves both tiles), then its multiplications and two hand-overs.  16384 tokens, 32 heads over 8: 2.0 to 2.2 ms with
 // the card's clock under its power limit, 1000 to 1100 TFLOP/s of what the mask leaves; 509 tokens behind 32000: 253 us, 1065.
-//  * Warp 0 loads keys and warp 2 values (TMA; a page's rows of a kv head are a box) into one ring of stages.  Warps 1 and 3 issue the
+//  * Warp 0 loads keys and warp 2 values (TMA; a page's rows of a kv head are a box), each into a ring of stages of its own: a wait's
+//    parity tells only neighbouring turns of a stage apart, so whoever loads one has to load every turn of it.  Warps 1 and 3 issue the
 //    multiplications of a tile each, and load its queries: issuing blocks while the tensor core is busy, and a commit costs it 78
 //    cycles, so one warp for both tiles with commits for the stages left it idle a third more.  Warps 4..7 and 8..11 are the softmax
 //    of the two tiles; they tell when a stage is read, from the completion of the scores behind it.
@@ -244,8 +245,23 @@ __device__ __forceinline__ void tmem_load16_at(uint32_t taddr, uint32_t* v) {
 template <int DP>
 struct PromptSizes {
   static constexpr uint32_t kTile = 128 * DP * 2;                   // bytes of a tile of queries, a block of keys or of values
-  static constexpr int kStages = DP == 128 ? 5 : 8;
+  static constexpr int kKeyStages = DP == 128 ? 3 : 4;
+  static constexpr int kValueStages = DP == 128 ? 2 : 4;
+  static constexpr int kStages = kKeyStages + kValueStages;
   static constexpr size_t kSmem = (2 + kStages) * kTile;   // and 3 KB of static variables: all that a block can have
+};
+
+// The turns of a ring of stages: the stage of the next one, and the parity that a wait for its copy takes.
+template <int FIRST, int STAGES>
+struct Ring {
+  int s = FIRST;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void step() {
+    if (++s == FIRST + STAGES) {
+      s = FIRST;
+      ph ^= 1u;
+    }
+  }
 };
 
 template <typename T, int DP>
@@ -254,6 +270,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     const __grid_constant__ PromptArgs P) {
   using Z = PromptSizes<DP>;
   constexpr int kStages = Z::kStages;
+  using Keys = Ring<0, Z::kKeyStages>;
+  using Values = Ring<Z::kKeyStages, Z::kValueStages>;
   constexpr uint32_t kHalf = 128 * 128;   // bytes of 64 columns of a tile: 128 rows of 128 bytes, swizzled
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], mma_done[2], tail_full;
@@ -379,7 +397,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const float c = fmaxf(fabsf(P.a.scale) * 1.4426950408889634f, 1e-30f);
     const bool leader = (warp & 3) == 0 && lane == 0;
     uint8_t* const mine_rows = smem_raw + x * Z::kTile + (warp & 3) * (Z::kTile / 4);   // 32 rows of the queries' place
-    int s_count = 0, o_count = 0, stage = 0, v_before = 0;
+    int s_count = 0, o_count = 0, v_before = 0;
+    Keys keys;
+    Values values;
     auto mend_rows = [&](const Piece& p, const TileRange& r, bool bad, int pos, int lo, int head, int token) {
       uint32_t rows = __ballot_sync(0xffffffffu, bad);
       if (__builtin_expect(rows == 0, 1)) return;
@@ -409,8 +429,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (!here && !r2.has(j)) continue;
         // The scores' completion tells that the multiplications are done with the keys of this block and the values of the one
         // before: one thread per tile gives the stages back.  (A commit of its own for each would hold the tensor core up by 78 cycles.)
-        const int k_stage = stage, v_stage = k_stage + 1 == kStages ? 0 : k_stage + 1;
-        stage = v_stage + 1 == kStages ? 0 : v_stage + 1;
+        const int k_stage = keys.s, v_stage = values.s;
+        keys.step();
+        values.step();
         if (!here) continue;   // the other tile's; this tile's issuing warp gives the stages back
         if (!(ok = wait_warp(s_full + x, s_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
         if (leader) {
@@ -553,7 +574,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     if (warp == 0 || warp == 2) {   // ------------------------------------------------------- loads: warp 0 keys, warp 2 values
       const bool values = warp == 2;
       const void* const map = values ? &VM : &KM;
-      int s = values, tails = 0, fills = 0;
+      const int ring_begin = values ? Z::kKeyStages : 0, ring_end = values ? kStages : Z::kKeyStages;
+      int s = ring_begin, tails = 0, fills = 0;
       uint32_t ph = 0;
       bool ok = true;
       constexpr int kHalves = DP / 64;
@@ -609,9 +631,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (elect_one()) mbar_arrive(full + s);
             __syncwarp();
           }
-          s += 2;   // the ring holds keys and values in turn
-          if (s >= kStages) {
-            s -= kStages;
+          if (++s == ring_end) {
+            s = ring_begin;
             ph ^= 1u;
           }
         }
@@ -622,21 +643,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int steps = P.dim16 / 16, x = warp >> 1;
       const uint32_t ts = tmem + x * 128, to = tmem + 256 + x * 128;
       const uint64_t q = smem_desc_sw128(base + x * Z::kTile);
-      int s = 0, q_count = 0, p_count = 0;
-      uint32_t ph = 0;
+      int q_count = 0, p_count = 0;
+      Keys keys;
+      Values values;
       bool ok = true, any = false;
       auto wait = [&](uint64_t* bar, int parity) -> bool {
         if (ok) ok = wait_warp(bar, parity, P.wait_limit, P.a.err, abort_flag);
         tc_fence_after();
         return ok;
-      };
-      auto next_stage = [&]() -> uint32_t {
-        const uint32_t stage = s;
-        if (++s == kStages) {
-          s = 0;
-          ph ^= 1u;
-        }
-        return stage;
       };
       uint64_t v = 0;   // the values of the block before
       auto weighted_sum = [&](bool fresh) {   // O (+)= P V
@@ -655,7 +669,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int j = p.j0; j < p.j1 && ok; ++j) {
           const bool here = r.has(j);
           if (!here && !r2.has(j)) continue;
-          const uint32_t k_ph = ph, k_stage = next_stage(), v_ph = ph, v_stage = next_stage();
+          const uint32_t k_ph = keys.ph, k_stage = keys.s, v_ph = values.ph, v_stage = values.s;
+          keys.step();
+          values.step();
           if (!here) {
             // The other tile's block, given back once it is there: the turns of a stage must not overtake a warp that waits on its
             // barriers, whose parity tells only neighbouring turns apart.
