@@ -741,6 +741,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int parity = 0; parity < 2; ++parity) mbar_wait(smem_addr(full + i), parity, P.a.err, 1u << 14);
     for (int x = 0; x < 2; ++x)
       for (int parity = 0; parity < 2; ++parity) mbar_wait(smem_addr(q_full + x), parity, P.a.err, 1u << 14);
+    for (int parity = 0; parity < 2; ++parity) mbar_wait(smem_addr(&tail_full), parity, P.a.err, 1u << 14);
   }
 }
 

@@ -188,3 +188,14 @@ def test_the_kernels_rings(dims):
 def test_one_ring_for_both_is_seen_to_fail():
     with pytest.raises(Overwritten):
         replay((5,), 1500, 3)
+
+
+def test_a_block_that_gives_up_waits_for_every_copy():
+    """Each barrier that copies are counted on is waited for before the block gives its shared memory back."""
+    text = open(os.path.join(ROOT, "lazyweights_b200", "csrc", "lw_attend_prompt.cu")).read()
+    kernel = text[text.index("    k_attend_prompt("):text.index(" k_attend_join(")]
+    on = set(re.findall(r"mbar_expect\((\w+)", kernel))
+    on |= set(re.findall(r"uint64_t\* const bar = cut \? &(\w+) : (\w+)", kernel)[0])
+    assert on - {"bar"} == {"full", "q_full", "tail_full"}
+    gives_up = kernel[kernel.index("if (abort_word"):]
+    assert all(re.search(r"mbar_wait\(smem_addr\(&?%s\b" % name, gives_up) for name in on - {"bar"})

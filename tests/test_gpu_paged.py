@@ -441,6 +441,29 @@ def test_a_lost_copy_ends_the_kernel(lw, prompt):
         lib.lw_debug_set(b"reset", 0)
 
 
+@pytest.mark.parametrize("window", [0, 50])
+def test_a_lost_copy_among_partly_seen_blocks(lw, window):
+    """The same where every block of positions is only partly seen, so that values are waited for by the warp that loads them."""
+    import torch
+    pr = problem([100] * 200, [100] * 200, 4, 2, 128, 16, "fp16")
+    cache = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+    args = [pr[n].cuda() for n in ("q", "table", "lens", "starts")]
+    want = cache.attend_prompt(*args, window=window)
+    torch.cuda.synchronize()
+    lib = lw.lib()
+    try:
+        for unit in (0, 1):
+            lib.lw_debug_set(b"wait_limit", 2000)
+            lib.lw_debug_set(b"drop_unit", unit)
+            cache.attend_prompt(*args, window=window)
+            torch.cuda.synchronize()
+            assert lib.lw_kernel_error() == 1
+            lib.lw_debug_set(b"reset", 0)
+            assert torch.equal(cache.attend_prompt(*args, window=window), want)
+    finally:
+        lib.lw_debug_set(b"reset", 0)
+
+
 # ------------------------------------------------------------------------------------------- graphs, streams, together
 
 
