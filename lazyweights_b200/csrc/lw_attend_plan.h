@@ -42,6 +42,10 @@ LW_HD long long floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
   return sum;
 }
 
+// The first position that the row at `pos` sees (window 0: all).  Any window >= 0 and any pos, those before position 0 too: the difference
+// is only taken where it is positive.
+LW_HD int window_begin(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
+
 struct PromptShape {
   int pair_tokens, window, lead;
 };
@@ -62,7 +66,7 @@ LW_HD PairRange pair_range(const PromptShape& s, const PromptSeq& q, int i) {
   const int t1 = q.rows - t0 < s.pair_tokens ? q.rows : t0 + s.pair_tokens;
   PairRange r;
   r.hi = p0 + t1;
-  r.lo = s.window > 0 && p0 + t0 - s.window + 1 > 0 ? p0 + t0 - s.window + 1 : 0;
+  r.lo = window_begin(p0 + t0, s.window);
   r.first = r.lo / kPosBlock;
   r.last = r.hi > r.lo ? (r.hi + kPosBlock - 1) / kPosBlock : r.first + 1;
   return r;
@@ -87,9 +91,8 @@ LW_HD long long units_before(const PromptShape& s, const PromptSeq& q, int i) {
   }
   if (whole > none) sum += floor_sum(whole - none, kPosBlock, T, p0 + (none + 1) * T + kPosBlock - 1);
   if (s.window > 0) {   // less the blocks before the window: first = floor((p0 - window + 1 + k T) / 128) where that is positive
-    const int b = p0 - s.window + 1;
-    int k1 = b < 0 ? (-b + T - 1) / T : 0;
-    if (whole > k1) sum -= floor_sum(whole - k1, kPosBlock, T, b + k1 * T);
+    const long long b = static_cast<long long>(p0) - s.window + 1, k1 = b < 0 ? (-b + T - 1) / T : 0;
+    if (whole > k1) sum -= floor_sum(static_cast<uint32_t>(whole - k1), kPosBlock, T, static_cast<uint32_t>(b + k1 * T));
   }
   return sum;
 }

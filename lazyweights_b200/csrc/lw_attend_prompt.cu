@@ -135,8 +135,7 @@ __device__ __forceinline__ TileRange tile_range(const PromptArgs& P, const Piece
   r.tokens = min(P.tile_tokens, p.s.q.rows - t0);
   r.p_first = p0 + t0;
   r.p_last = p0 + t0 + r.tokens - 1;
-  const int lo = P.a.window > 0 ? max(0, r.p_first - P.a.window + 1) : 0;
-  r.first = max(p.j0, lo / kPosBlock);
+  r.first = max(p.j0, window_begin(r.p_first, P.a.window) / kPosBlock);
   r.last = min(p.j1, (r.p_last + kPosBlock) / kPosBlock);
   if (r.tokens <= 0 || r.p_last < 0) r.last = r.first = 0;
   return r;
@@ -406,7 +405,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const PairRange pr = pair_range(shape, p.s.q, p.t0 / shape.pair_tokens);
       __syncwarp();
       if (!values_not_finite<T>(P, p.b, p.h, max(0, r.p_first + 1), pr.hi) &&
-          !(P.a.window > 0 && values_not_finite<T>(P, p.b, p.h, pr.lo, max(0, r.p_last - P.a.window + 1)))) return;
+          !(P.a.window > 0 && values_not_finite<T>(P, p.b, p.h, pr.lo, window_begin(r.p_last, P.a.window)))) return;
       for (; rows; rows &= rows - 1) {
         const int src = __ffs(rows) - 1;
         const int row_pos = __shfl_sync(0xffffffffu, pos, src), row_lo = __shfl_sync(0xffffffffu, lo, src);
@@ -421,7 +420,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const TileRange r = tile_range(P, p, x), r2 = tile_range(P, p, x ^ 1);
       const bool mine = token < min(r.tokens, P.tile_tokens);
       const int pos = mine ? r.p_first + token : -1;
-      const int lo = P.a.window > 0 ? max(0, pos - P.a.window + 1) : 0;
+      const int lo = window_begin(pos, P.a.window);
       const bool idle = !__any_sync(0xffffffffu, mine);
       float m = -INFINITY, l = 0.f;
       for (int j = p.j0; j < p.j1; ++j) {
@@ -800,10 +799,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
   if (__builtin_expect(!__syncthreads_or(rows != 0), 1)) return;   // the four warps share the rows, a quarter of the dimensions each
   const int kh = n.head0 / P.group;
   if (!values_not_finite<T>(P, n.b, kh, max(0, n.position + 1), n.position + n.rows) &&
-      !(P.a.window > 0 && values_not_finite<T>(P, n.b, kh, max(0, n.position - P.a.window + 1), max(0, n.position + n.rows - P.a.window)))) return;
+      !(P.a.window > 0 && values_not_finite<T>(P, n.b, kh, window_begin(n.position, P.a.window), window_begin(n.position + n.rows - 1, P.a.window)))) return;
   for (; rows; rows &= rows - 1) {   // several warps may write the same row, all of them the same
     const int src = __ffs(rows) - 1, row_t = __shfl_sync(0xffffffffu, t, src), pos = n.position + row_t;
-    single_row<T>(P, n.b, kh, n.row0 + row_t, n.head0 + __shfl_sync(0xffffffffu, head, src), P.a.window > 0 ? max(0, pos - P.a.window + 1) : 0, pos);
+    single_row<T>(P, n.b, kh, n.row0 + row_t, n.head0 + __shfl_sync(0xffffffffu, head, src), window_begin(pos, P.a.window), pos);
   }
 }
 

@@ -206,6 +206,7 @@ static int check_cache_device(const PagedCache* c) {
 static int check_sequences(const char* what, const int* starts, const int* lens, const int* table, int n_seqs, int table_cols,
                            long long table_stride, int n_rows, bool starts_needed) {
   if (n_seqs < 1 || n_rows < 1) return refuse(what, "needs at least one sequence and one row");
+  if (n_rows > 1 << 30) return refuse(what, "at most 2^30 rows");   // positions of rows before position 0 are counted in 32 bits
   if (!lens || !table || (starts_needed && !starts)) return refuse(what, "null pointer");
   if (table_cols < 1 || table_stride < table_cols) return refuse(what, "the page table has no columns, or rows closer than that");
   if (!starts && n_rows < n_seqs) return refuse(what, "fewer rows than sequences");

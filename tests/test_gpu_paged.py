@@ -127,6 +127,27 @@ def test_prompt_window(lw, window):
     check_attention(lw, problem([n for n, _ in lens], [m for _, m in lens], 4, 2, 128, 32, "fp16", seed=window), window=window)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 128, 2 ** 30])
+def test_windows_without_an_end(lw, window):
+    """A window that nothing fills is none, up to the largest, also for rows before position 0."""
+    import torch
+    lens = [(200, 200), (1000, 70), (1, 1), (300, 300)]
+    pr = problem([n for n, _ in lens], [m for _, m in lens], 4, 2, 64, 16, "fp16", seed=6)
+    pr["starts"] = torch.tensor([0, 200, 270, 271, 591], dtype=torch.int32)      # 20 rows more than the last one has positions
+    pr["q"] = torch.randn(591, 4, 64, generator=torch.Generator().manual_seed(1)).half()
+    cache = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+    args = [pr[n].cuda() for n in ("q", "table", "lens", "starts")]
+    got = cache.attend_prompt(*args, window=window)
+    assert torch.equal(got, cache.attend_prompt(*args)) and (got[271:291] == 0).all()
+    for m in (4, 64):      # tiles of other numbers of tokens
+        sub = args[0][:, :1].expand(-1, m, -1).contiguous()
+        assert torch.equal(cache.attend_prompt(sub, *args[1:], window=window), cache.attend_prompt(sub, *args[1:]))
+    one = [args[0][:4].contiguous(), *args[1:3]]
+    assert torch.equal(cache.attend(*one, window=window), cache.attend(*one))
+    keep = torch.cat((torch.arange(271), torch.arange(291, 591)))
+    check_attention(lw, dict(pr, q=pr["q"][keep], starts=torch.tensor([0, 200, 270, 271, 571], dtype=torch.int32)), window=window)
+
+
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.25, 2.0])
 def test_scales(lw, scale):
     """Equal weights, sharp maxima (scores of a few dozen), a negative scale."""

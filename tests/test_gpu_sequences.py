@@ -151,3 +151,19 @@ def test_refusals(tmp_path):
         with pytest.raises(ValueError):
             b.forward_seqs([ids], [4, 4], [[0]])
         assert np.isfinite(b.forward_seqs([ids], [4], [[0]])).all() and b.kernel_error() == 0
+
+
+@pytest.mark.gpu
+def test_the_largest_window_is_none(tmp_path):
+    helpers.build_library()
+    import lazyweights_b200 as lw
+    rng = np.random.default_rng(5)
+    ids = [rng.integers(0, 256, n).astype(np.int32) for n in (40, 7)]
+    with lw.Bundle(_model(tmp_path, 8, 2, 64)[0], max_ctx=128, max_batch=64) as b:
+        b.open_pages(8, 16)
+        table = [[0, 2, 4, 6], [1, 3, 5, 7]]
+        got = []
+        for window in (0, 2 ** 31 - 1):
+            b.set_window(window)
+            got.append((b.forward_seqs(ids, [40, 7], table), b.forward_seqs([i[:1] for i in ids], [41, 8], table)))
+        assert all(np.array_equal(x, y) for x, y in zip(*got)) and b.kernel_error() == 0

@@ -121,3 +121,8 @@ def test_python_refuses_pools_on_the_host(nat):
         lw.PagedCache(torch.zeros(2, 2, 8, 64, dtype=torch.float16), torch.zeros(2, 2, 8, 64, dtype=torch.float16))
     with pytest.raises(ValueError):
         lw.PagedCache(torch.zeros(2, 2, 8, 64), torch.zeros(2, 2, 8, 64))
+
+
+def test_rows_beyond_32_bits_of_positions_are_refused(nat):
+    for fn, base in (("lw_cache_append", APPEND), ("lw_cache_attend_prompt", PROMPT)):
+        refused(nat, fn, base, dict(rows=(1 << 30) + 1))
