@@ -95,7 +95,8 @@ int rt_forward(void* handle, const int* ids, int n, float* logits, int all_logit
 int rt_decode_greedy(void* handle, int first_token, int n, int* out);
 
 /* Several sequences in one pass (additions; the reference's runtime holds one sequence).  rt_pages gives the handle a paged cache of
- * its own, n_pages pages of page_size positions (a multiple of 8) in every layer, empty; calling it again replaces the cache.
+ * its own, n_pages pages of page_size positions (a multiple of 8; 2^31 - 1 positions at most in all) in every layer, empty; calling it
+ * again replaces the cache.
  * rt_forward_seqs runs the new tokens of n_seqs sequences through the decoder: sequence b's are ids[starts[b]] ..
  * ids[starts[b + 1] - 1] (starts[0] = 0; one at least per sequence, max_batch at most in all), the last of its lens[b] positions;
  * its pages are table[b * table_cols + 0 ..], which the caller gives out - two sequences may share the pages of a common

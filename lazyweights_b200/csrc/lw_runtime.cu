@@ -1486,6 +1486,10 @@ int rt_pages(void* handle, int n_pages, int page_size) {
     set_error("rt_pages: no model runtime in this handle, no pages, or a page size that is no multiple of 8");
     return kErrArg;
   }
+  if (static_cast<long long>(n_pages) * page_size > 0x7fffffffll) {   // the bytes of all layers then fit 64 bits for every model that can be opened
+    set_error("rt_pages: more than 2^31 - 1 positions in all");
+    return kErrArg;
+  }
   Runtime* R = M->rt;
   if (const int rc = check_device(M)) return rc;
   if (R->tp_world > 1) {

@@ -167,3 +167,20 @@ def test_the_largest_window_is_none(tmp_path):
             b.set_window(window)
             got.append((b.forward_seqs(ids, [40, 7], table), b.forward_seqs([i[:1] for i in ids], [41, 8], table)))
         assert all(np.array_equal(x, y) for x, y in zip(*got)) and b.kernel_error() == 0
+
+
+@pytest.mark.gpu
+def test_a_pool_beyond_32_bits_of_positions_is_refused(tmp_path):
+    """By its size, before anything is allocated or freed: a product of its bytes could wrap to a small number."""
+    helpers.build_library()
+    import lazyweights_b200 as lw
+    from lazyweights_b200 import _native as nat
+    ids = np.arange(5, dtype=np.int32)
+    with lw.Bundle(_model(tmp_path, 8, 2, 64)[0], max_ctx=64, max_batch=8) as b:
+        b.open_pages(3, 16)
+        want = b.forward_seqs([ids], [5], [[1]])
+        for pages, size in ((2 ** 31 - 1, 65536), (2 ** 28, 8), (2 ** 15, 65536)):
+            with pytest.raises(lw.LwError) as e:
+                b.open_pages(pages, size)
+            assert e.value.status == nat.LW_ERR_ARG
+        assert np.array_equal(b.forward_seqs([ids], [5], [[1]]), want)      # the cache that was there serves on
