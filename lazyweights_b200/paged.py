@@ -25,6 +25,13 @@ def _codes(torch):
     return _CODES
 
 
+def _window(window):
+    """ctypes would cut it to 32 bits."""
+    if not 0 <= window < 1 << 31:
+        raise ValueError("window must be 0 (all positions) .. 2^31 - 1, not %r" % (window,))
+    return window
+
+
 class PagedCache:
     """Pools k_pages and v_pages [pages, kv_heads, page_size, head_dim], CUDA fp16 or bf16, of the same strides (any multiples of
     eight, head_dim contiguous: a pool with the heads inside the positions is passed transposed).  The tensors are kept alive."""
@@ -148,8 +155,8 @@ class PagedCache:
         _, _, ot, oh = self._rows(out, "out", n, heads)
         space, size = self._workspace(torch, heads, 0)
         rc = self._lib.lw_cache_attend(self._h, q.data_ptr(), qt, qh, n, heads, lens.data_ptr(), table.data_ptr(), cols, tstride,
-                                       self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(), ot, oh, space.data_ptr(), size,
-                                       _stream(torch, self._index))
+                                       self.head_dim ** -0.5 if scale is None else scale, _window(window), out.data_ptr(), ot, oh,
+                                       space.data_ptr(), size, _stream(torch, self._index))
         if rc < 0:
             nat.check(rc)
         return out
@@ -167,7 +174,7 @@ class PagedCache:
         _, _, ot, oh = self._rows(out, "out", rows, heads)
         space, size = self._workspace(torch, heads, 1)
         rc = self._lib.lw_cache_attend_prompt(self._h, q.data_ptr(), qt, qh, rows, heads, starts.data_ptr(), lens.data_ptr(), table.data_ptr(), n, cols,
-                                              tstride, self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(), ot, oh,
+                                              tstride, self.head_dim ** -0.5 if scale is None else scale, _window(window), out.data_ptr(), ot, oh,
                                               space.data_ptr(), size, _stream(torch, self._index))
         if rc < 0:
             nat.check(rc)

@@ -32,6 +32,19 @@ def _stream(torch, device_index):
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
+def _int32(values, what):
+    """A contiguous int32 array of these whole numbers; a conversion that would change one (2**32 + 4 to 4) is refused."""
+    given = np.asarray(values)
+    try:
+        with np.errstate(invalid="ignore"):
+            out = np.ascontiguousarray(given, np.int32)
+    except OverflowError:
+        out = None
+    if out is None or given.dtype != np.int32 and not np.array_equal(given, out):
+        raise ValueError("%s must be whole numbers of 32 bits" % what)
+    return out
+
+
 class _Handle:
     def __init__(self, ptr):
         if not ptr:
@@ -257,16 +270,16 @@ class Bundle(_Handle):
 
     def open_pages(self, n_pages, page_size=16):
         """rt_pages: a paged cache for several sequences, `n_pages` pages of `page_size` positions in every layer."""
-        nat.check(nat.lib().rt_pages(self._h, int(n_pages), int(page_size)))
+        nat.check(nat.lib().rt_pages(self._h, *_int32((n_pages, page_size), "n_pages and page_size").tolist()))
 
     def forward_seqs(self, ids, lens, table):
         """rt_forward_seqs: one pass over the new tokens of several sequences.  ids: a list of their token arrays, lens: their lengths
         with the new tokens, table: [n, columns] their pages.  Returns the logits of every sequence's last token [n, vocab] (host
         float32)."""
-        parts = [np.ascontiguousarray(i, np.int32).reshape(-1) for i in ids]
+        parts = [_int32(i, "ids").reshape(-1) for i in ids]
         starts = np.cumsum([0] + [p.size for p in parts]).astype(np.int32)
         flat = np.concatenate(parts) if parts else np.zeros(0, np.int32)
-        lens, table = np.ascontiguousarray(lens, np.int32).reshape(-1), np.ascontiguousarray(table, np.int32)
+        lens, table = _int32(lens, "lens").reshape(-1), _int32(table, "table")
         if table.ndim != 2 or table.shape[0] != len(parts) or lens.size != len(parts):
             raise ValueError("forward_seqs wants a length and a row of the page table per sequence")
         out = np.empty((len(parts), nat.lib().rt_vocab(self._h)), np.float32)

@@ -580,6 +580,17 @@ def test_python_refusals(lw):
         lw.PagedCache(k[:, :, :12].contiguous(), v[:, :, :12].contiguous())       # page size
 
 
+def test_windows_that_do_not_fit_are_refused(lw):
+    pr = problem([40, 40], [2, 2], 4, 2, 64, 16, "fp16")
+    cache = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+    q, table, lens, starts = (pr[n].cuda() for n in ("q", "table", "lens", "starts"))
+    for window in (-1, 2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(ValueError):
+            cache.attend(q[:2], table, lens, window=window)
+        with pytest.raises(ValueError):
+            cache.attend_prompt(q, table, lens, starts, window=window)
+
+
 def test_prompt_then_tokens(lw):
     """A whole use: packed prompts are appended and attended to, in two pieces for one of them, then tokens one by one."""
     import torch

@@ -184,3 +184,19 @@ def test_a_pool_beyond_32_bits_of_positions_is_refused(tmp_path):
                 b.open_pages(pages, size)
             assert e.value.status == nat.LW_ERR_ARG
         assert np.array_equal(b.forward_seqs([ids], [5], [[1]]), want)      # the cache that was there serves on
+
+
+@pytest.mark.gpu
+def test_numbers_that_do_not_fit_are_refused(tmp_path):
+    helpers.build_library()
+    import lazyweights_b200 as lw
+    ids = np.arange(4, dtype=np.int64)
+    with lw.Bundle(_model(tmp_path, 8, 2, 64)[0], max_ctx=64, max_batch=8) as b:
+        with pytest.raises(ValueError):
+            b.open_pages(2 ** 32 + 3, 16)
+        b.open_pages(3, 16)
+        for args in (([ids + 2 ** 32], [4], [[0]]), ([ids], np.array([2 ** 32 + 4]), [[0]]), ([ids], [4], np.array([[2 ** 32]])), ([ids + 0.5], [4], [[0]])):
+            with pytest.raises(ValueError):
+                b.forward_seqs(*args)
+        want = b.forward_seqs([ids.astype(np.int32)], [4], [[0]])
+        assert np.array_equal(b.forward_seqs([ids], np.array([4]), np.array([[0]])), want)

@@ -126,3 +126,22 @@ def test_python_refuses_pools_on_the_host(nat):
 def test_rows_beyond_32_bits_of_positions_are_refused(nat):
     for fn, base in (("lw_cache_append", APPEND), ("lw_cache_attend_prompt", PROMPT)):
         refused(nat, fn, base, dict(rows=(1 << 30) + 1))
+
+
+@pytest.mark.parametrize("window", [-1, 2 ** 31, 2 ** 32 + 5, 2 ** 64])
+def test_python_windows_that_do_not_fit(window):
+    from lazyweights_b200 import paged
+    with pytest.raises(ValueError):
+        paged._window(window)
+    assert paged._window(2 ** 31 - 1) == 2 ** 31 - 1 and paged._window(0) == 0
+
+
+def test_python_numbers_that_do_not_fit():
+    import numpy as np
+    from lazyweights_b200.runtime import _int32
+    for good in ([1, 2], np.array([[3, -4]]), np.array([5.0, 6.0]), np.zeros(0), np.arange(3, dtype=np.uint8), np.arange(4, dtype=np.int32)[::2]):
+        out = _int32(good, "x")
+        assert out.dtype == np.int32 and out.flags.c_contiguous and np.array_equal(out, good)
+    for bad in ([2 ** 31], [2 ** 32 + 4], np.array([2 ** 32 + 4]), np.array([-2 ** 31 - 1]), [2 ** 70], [1.5], [float("nan")], np.array([2 ** 64 - 1], np.uint64)):
+        with pytest.raises(ValueError):
+            _int32(bad, "x")
