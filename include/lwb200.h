@@ -338,7 +338,8 @@ int lw_cache_attend(void* cache, const void* q, long long q_token_stride, long l
                     long long out_token_stride, long long out_head_stride, void* workspace, long long workspace_bytes, void* stream);
 
 /* The same for the rows of packed prompts, or of pieces of prompts whose beginnings are in the pages already: the row at position p
- * sees max(0, p - window + 1) .. p.  A row before position 0 sees nothing and gives zeros; rows of no sequence are left alone. */
+ * sees max(0, p - window + 1) .. p.  A row before position 0 sees nothing and gives zeros; rows of no sequence are left alone.  A row
+ * that sees positions, but only with scores of -inf, is NaN (here and in lw_cache_attend). */
 int lw_cache_attend_prompt(void* cache, const void* q, long long q_token_stride, long long q_head_stride, int n_rows, int n_heads,
                            const int* starts, const int* lens, const int* table, int n_seqs, int table_cols, long long table_stride,
                            float scale, int window, void* out, long long out_token_stride, long long out_head_stride, void* workspace,

@@ -182,7 +182,7 @@ __device__ __noinline__ void single_row(const PromptArgs& P, int b, int kh, long
     for (int i = 0; i < 4; ++i) s = fmaf(number(q, i), number(k, i), s);
     for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
     s *= P.a.scale * 1.4426950408889634f;
-    const float m2 = fmaxf(m, s), keep = exp2_fast(m - m2), w = exp2_fast(s - m2);
+    const float m2 = fmaxf(m, s), ref = m2 == -INFINITY ? 0.f : m2, keep = exp2_fast(m - ref), w = exp2_fast(s - ref);
     m = m2;
     l = l * keep + w;
     for (int i = 0; i < 4; ++i) o[i] = o[i] * keep + w * number(v, i);
@@ -784,7 +784,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
     }
   }
   T* out = static_cast<T*>(P.a.out) + static_cast<long long>(n.row0 + t) * P.a.out_token + static_cast<long long>(n.head0 + head) * P.a.out_head;
-  const float f = l == 0.f ? 0.f : 1.f / l;
+  const float f = n.position + t < 0 ? 0.f : 1.f / l;   // a row before position 0 gives zeros; one whose scores are all -inf NaN, as in a pair that is whole
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {

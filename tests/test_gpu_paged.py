@@ -204,6 +204,42 @@ def test_infinities_and_nan_in_sight_show(lw):
     assert torch.isnan(one[0]).all() and torch.isfinite(one[1]).all()
 
 
+@pytest.mark.parametrize("value", [1.0, float("inf")])
+@pytest.mark.parametrize("length,new,low", [(200, 200, 150), (300, 70, 250), (6000, 30, 5980), (6000, 30, 3000), (700, 700, 130), (40000, 5, 39999)])
+def test_scores_of_minus_infinity(lw, length, new, low, value):
+    """Keys before position `low` whose scores are -inf: rows that see no other are NaN, whether the work on them is split or not,
+    and the others are as if those positions were not there; also beside an infinite value that only the last row sees."""
+    import torch
+    from tests import paged_ref as ref
+    pr = problem([length, 100], [new, 100], 4, 2, 64, 16, "fp16", seed=length)
+    pr["q"][:, :, 0] = 1.0
+    keys, v = (ref.load(pr[n], pr["table"], 0, length) for n in "kv")
+    keys[:low, :, 0] = -float("inf")
+    v[length - 1, :, 5] = value
+    ref.store(pr["k"], pr["table"], 0, 0, keys)
+    ref.store(pr["v"], pr["table"], 0, 0, v)
+    cache = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+    args = [pr[n].cuda() for n in ("q", "table", "lens", "starts")]
+    out = cache.attend_prompt(*args).cpu().double()
+    first = length - new
+    none = max(0, low - first)                 # rows that see positions before `low` alone
+    assert torch.isnan(out[:none]).all() and torch.isfinite(out[new:]).all()
+    # without those positions: the rest of the sequence, seen from the same places
+    clean = torch.where(torch.isfinite(v), v, torch.zeros((), dtype=torch.float64))
+    want, bound, _ = ref.attend(pr["q"][none:new], keys[low:], clean[low:], torch.arange(first + none, length) - low, 64 ** -0.5, 0)
+    good = ((out[none:new] - want).abs() <= bound)
+    if value != 1.0:
+        assert not torch.isfinite(out[new - 1, :, 5]).any()
+        good[-1, :, 5] = True
+    assert good.all()
+    for last in (low, length):                 # one token: all scores -inf, or not
+        one = cache.attend(args[0][new - 1:new].contiguous(), args[1][:1], torch.full_like(args[2][:1], last)).cpu()
+        if last == low:
+            assert torch.isnan(one).all()
+        else:
+            assert ((one.double() - want[-1]).abs() <= bound[-1])[:, :, :5].all()
+
+
 @pytest.mark.parametrize("window", [0, 40])
 @pytest.mark.parametrize("heads,length,new", [(2, 200, 200), (4, 300, 70), (2, 6000, 30)])
 def test_values_out_of_sight_do_not_show(lw, heads, length, new, window):
