@@ -332,7 +332,8 @@ long long lw_cache_workspace(void* cache, int n_heads, int prompt);
 /* Attention of one new token per sequence: out[b][h] = sum_j softmax_j(scale q[b][h] . k_j) v_j over the positions
  * max(0, lens[b] - window) <= j < lens[b] (window 0: from 0).  Query head h reads kv head h / (n_heads / n_kv_heads), at most 128
  * query heads per kv head.  q and out in
- * the cache's type, rows and heads on 16-byte boundaries.  A sequence of length 0 gives zeros. */
+ * the cache's type, rows and heads on 16-byte boundaries; out may be q itself, with the same strides.  A sequence of length 0 gives
+ * zeros. */
 int lw_cache_attend(void* cache, const void* q, long long q_token_stride, long long q_head_stride, int n_seqs, int n_heads, const int* lens,
                     const int* table, int table_cols, long long table_stride, float scale, int window, void* out,
                     long long out_token_stride, long long out_head_stride, void* workspace, long long workspace_bytes, void* stream);

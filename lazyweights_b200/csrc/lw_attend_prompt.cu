@@ -399,19 +399,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     int s_count = 0, o_count = 0, v_before = 0;
     Keys keys;
     Values values;
-    auto mend_rows = [&](const Piece& p, const TileRange& r, bool bad, int pos, int lo, int head, int token) {
-      uint32_t rows = __ballot_sync(0xffffffffu, bad);
-      if (__builtin_expect(rows == 0, 1)) return;
+    auto rows_to_mend = [&](const Piece& p, const TileRange& r, bool bad) -> uint32_t {
+      const uint32_t rows = __ballot_sync(0xffffffffu, bad);
+      if (__builtin_expect(rows == 0, 1)) return 0u;
       const PairRange pr = pair_range(shape, p.s.q, p.t0 / shape.pair_tokens);
       __syncwarp();
       if (!values_not_finite<T>(P, p.b, p.h, max(0, r.p_first + 1), pr.hi) &&
-          !(P.a.window > 0 && values_not_finite<T>(P, p.b, p.h, pr.lo, window_begin(r.p_last, P.a.window)))) return;
-      for (; rows; rows &= rows - 1) {
-        const int src = __ffs(rows) - 1;
-        const int row_pos = __shfl_sync(0xffffffffu, pos, src), row_lo = __shfl_sync(0xffffffffu, lo, src);
-        single_row<T>(P, p.b, p.h, p.s.row0 + p.t0 + x * P.tile_tokens + __shfl_sync(0xffffffffu, token, src),
-                      p.h * P.group + __shfl_sync(0xffffffffu, head, src), row_lo, row_pos);
-      }
+          !(P.a.window > 0 && values_not_finite<T>(P, p.b, p.h, pr.lo, window_begin(r.p_last, P.a.window)))) return 0u;
+      return rows;
     };
     bool ok = true;
     while (walk.left > 0 && ok) {
@@ -538,6 +533,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
         }
       }
+      uint32_t mend = 0;
       if (r.none() && p.begins && p.ends) {   // rows that see nothing
         if (mine)
           for (int d = 0; d < P.a.pool.Dh; d += 8)
@@ -546,7 +542,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       } else if (!idle && p.begins && p.ends) {
         // Row by row through the place of this tile's queries: a warp's store covers whole rows, not 16 bytes of 32 rows each, which
         // kept the load/store unit busy for 4000 cycles per pair.
-        const uint32_t rows = __ballot_sync(0xffffffffu, mine);
+        mend = rows_to_mend(p, r, check != 0.f && pos >= 0 && !not_finite(l));
+        const uint32_t rows = __ballot_sync(0xffffffffu, mine) & ~mend;   // those to be computed again are left: their queries may lie there
         const unsigned long long my_out = reinterpret_cast<unsigned long long>(static_cast<T*>(P.a.out) + static_cast<long long>(p.s.row0 + p.t0 + x * P.tile_tokens + token) * P.a.out_token +
                                                                               static_cast<long long>(p.h * P.group + head) * P.a.out_head);
         __syncwarp();
@@ -565,7 +562,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(q_empty + x);
       }
-      if (!idle && p.begins && p.ends) mend_rows(p, r, check != 0.f && pos >= 0 && !r.none() && !not_finite(l), pos, lo, head, token);
+      for (; mend; mend &= mend - 1) {
+        const int src = __ffs(mend) - 1;
+        const int row_pos = __shfl_sync(0xffffffffu, pos, src), row_lo = __shfl_sync(0xffffffffu, lo, src);
+        single_row<T>(P, p.b, p.h, p.s.row0 + p.t0 + x * P.tile_tokens + __shfl_sync(0xffffffffu, token, src),
+                      p.h * P.group + __shfl_sync(0xffffffffu, head, src), row_lo, row_pos);
+      }
       tc_fence_before();   // the next P is announced after these reads of O
     }
   } else {
@@ -787,21 +789,27 @@ __global__ void __launch_bounds__(kJoinThreads) k_attend_join(const __grid_const
   const float f = n.position + t < 0 ? 0.f : 1.f / l;   // a row before position 0 gives zeros; one whose scores are all -inf NaN, as in a pair that is whole
   bool bad = false;
 #pragma unroll
+  for (int i = 0; i < kSteps; ++i)
+    if (mine && (i * kWarps + warp) * 4 < P.a.pool.Dh) bad |= not_finite(o[i].x) || not_finite(o[i].y) || not_finite(o[i].z) || not_finite(o[i].w);
+  // as in k_attend_prompt, for all rows of the pair that this block holds: the four warps share them, a quarter of the dimensions each
+  uint32_t mend = __ballot_sync(0xffffffffu, bad && !not_finite(l));
+  const int kh = n.head0 / P.group;
+  if (__builtin_expect(__syncthreads_or(mend != 0), 0)) {
+    __shared__ uint32_t s_mend[kWarps];
+    if ((threadIdx.x & 31) == 0) s_mend[warp] = mend;
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w) mend |= s_mend[w];
+    if (!values_not_finite<T>(P, n.b, kh, max(0, n.position + 1), n.position + n.rows) &&
+        !(P.a.window > 0 && values_not_finite<T>(P, n.b, kh, window_begin(n.position, P.a.window), window_begin(n.position + n.rows - 1, P.a.window)))) mend = 0;
+  }
+#pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int d = (i * kWarps + warp) * 4;
-    if (mine && d < P.a.pool.Dh) {
-      *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(o[i].x * f, o[i].y * f), pack2<T>(o[i].z * f, o[i].w * f));
-      bad |= not_finite(o[i].x) || not_finite(o[i].y) || not_finite(o[i].z) || not_finite(o[i].w);
-    }
+    if (mine && d < P.a.pool.Dh && !(mend >> (threadIdx.x & 31) & 1u)) *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(o[i].x * f, o[i].y * f), pack2<T>(o[i].z * f, o[i].w * f));
   }
-  // as in k_attend_prompt, for all rows of the pair that this warp holds
-  uint32_t rows = __ballot_sync(0xffffffffu, bad && !not_finite(l));
-  if (__builtin_expect(!__syncthreads_or(rows != 0), 1)) return;   // the four warps share the rows, a quarter of the dimensions each
-  const int kh = n.head0 / P.group;
-  if (!values_not_finite<T>(P, n.b, kh, max(0, n.position + 1), n.position + n.rows) &&
-      !(P.a.window > 0 && values_not_finite<T>(P, n.b, kh, window_begin(n.position, P.a.window), window_begin(n.position + n.rows - 1, P.a.window)))) return;
-  for (; rows; rows &= rows - 1) {   // several warps may write the same row, all of them the same
-    const int src = __ffs(rows) - 1, row_t = __shfl_sync(0xffffffffu, t, src), pos = n.position + row_t;
+  for (int i = 0; mend; mend &= mend - 1, ++i) {   // a warp each
+    if ((i & (kWarps - 1)) != warp) continue;
+    const int src = __ffs(mend) - 1, row_t = __shfl_sync(0xffffffffu, t, src), pos = n.position + row_t;
     single_row<T>(P, n.b, kh, n.row0 + row_t, n.head0 + __shfl_sync(0xffffffffu, head, src), window_begin(pos, P.a.window), pos);
   }
 }

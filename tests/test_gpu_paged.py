@@ -271,6 +271,26 @@ def test_values_out_of_sight_do_not_show(lw, heads, length, new, window):
     assert torch.equal(~torch.isfinite(one[0]), shows[-1]) and torch.isfinite(one[1]).all()
 
 
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("heads,length,new", [(2, 200, 200), (4, 300, 70), (2, 6000, 30), (1, 6000, 300)])
+def test_results_in_the_place_of_the_queries(lw, heads, length, new, window):
+    """out = q gives the same bits, also for rows that are computed again beside values that are not finite."""
+    import torch
+    from tests import paged_ref as ref
+    for value in (1.0, float("inf")):
+        pr = problem([length, 100], [new, 100], heads, 1, 64, 16, "fp16", seed=heads)
+        v = ref.load(pr["v"], pr["table"], 0, length)
+        v[length - 1, 0, 5] = v[length - new // 2, 0, 9] = value
+        ref.store(pr["v"], pr["table"], 0, 0, v)
+        cache = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+        q, *args = [pr[n].cuda() for n in ("q", "table", "lens", "starts")]
+        for call, x, more in ((cache.attend_prompt, q, args), (cache.attend, q[:2].contiguous(), args[:2])):
+            want = call(x, *more, window=window)
+            same = x.clone()
+            call(same, *more, window=window, out=same)
+            assert torch.equal(same.view(torch.int16), want.view(torch.int16))
+
+
 def test_strided_queries_and_results(lw):
     """Queries inside the rows of a fused product, results into a slice of a wider tensor."""
     import torch
