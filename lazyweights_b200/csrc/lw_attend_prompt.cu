@@ -146,26 +146,39 @@ __device__ __forceinline__ TileRange tile_range(const PromptArgs& P, const Piece
 // its sum of weights is, the positions that the tile multiplied but some of its rows do not see are looked through, and if one
 // holds such a value the rows are computed again, one by one (a warp each time; the ordinary path pays a comparison per result).
 
-// The values of position p of kv head kh, this lane's four dimensions; zeros past the head and for a bad page.
-template <typename T>
-__device__ __forceinline__ uint2 four_of(const PromptArgs& P, const void* pool, int b, int kh, int p, int lane) {
+// Where position p of kv head kh lies in the pools; -1 for a bad page, whose keys and values are zeros.
+__device__ __forceinline__ long long place_of(const PromptArgs& P, int b, int kh, int p) {
   const int column = p / P.a.pool.page_size, page = P.a.seq.table[b * P.a.seq.table_stride + column];
-  if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(P.a.pool.n_pages) || lane * 4 >= P.a.pool.Dh) return make_uint2(0u, 0u);
-  return *reinterpret_cast<const uint2*>(static_cast<const T*>(pool) + page * P.a.pool.page_stride + kh * P.a.pool.head_stride +
-                                         (p - column * P.a.pool.page_size) * P.a.pool.token_stride + lane * 4);
+  if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(P.a.pool.n_pages)) return -1;
+  return page * P.a.pool.page_stride + kh * P.a.pool.head_stride + (p - column * P.a.pool.page_size) * P.a.pool.token_stride;
 }
+// This lane's four dimensions there; zeros past the head.  Loaded from somewhere in any case, so that loads need not wait for a branch.
+template <typename T>
+__device__ __forceinline__ uint2 four_of(const PromptArgs& P, const void* pool, long long at, int lane) {
+  const int d = lane * 4 < P.a.pool.Dh ? lane * 4 : 0;
+  uint2 v = *reinterpret_cast<const uint2*>(static_cast<const T*>(pool) + (at < 0 ? 0 : at) + d);
+  if (at < 0 || d != lane * 4) v = make_uint2(0u, 0u);
+  return v;
+}
+constexpr int kAtOnce = 8;   // positions whose loads a warp has in flight; the places of 32 are looked up together, a lane each
 template <typename T>
 __device__ __noinline__ bool values_not_finite(const PromptArgs& P, int b, int kh, int from, int to) {
   constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   const int lane = threadIdx.x & 31;
-  bool bad = false;
-  for (int p = from; p < to; ++p) {
-    const uint2 v = four_of<T>(P, P.a.pool.v, b, kh, p, lane);
-    for (int k = 0; k < 4; ++k) bad |= ((((k & 2) ? v.y : v.x) >> (16 * (k & 1))) & kExponent) == kExponent;
+  for (int p0 = from; p0 < to; p0 += 32) {
+    const long long at = p0 + lane < to ? place_of(P, b, kh, p0 + lane) : -1;
+    bool bad = false;
+#pragma unroll kAtOnce
+    for (int i = 0; i < 32; ++i) {
+      const uint2 v = four_of<T>(P, P.a.pool.v, __shfl_sync(0xffffffffu, at, i), lane);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) bad |= ((((k & 2) ? v.y : v.x) >> (16 * (k & 1))) & kExponent) == kExponent;
+    }
+    if (__any_sync(0xffffffffu, bad)) return true;
   }
-  return __any_sync(0xffffffffu, bad);
+  return false;
 }
-// Attention of one row over positions lo .. pos, by a warp.
+// Attention of one row over positions lo .. pos, by a warp.  28 rows at 100000 positions, seven to a warp: 107 ms (position by position 374).
 template <typename T>
 __device__ __noinline__ void single_row(const PromptArgs& P, int b, int kh, long long row, int head, int lo, int pos) {
   const int lane = threadIdx.x & 31;
@@ -174,18 +187,44 @@ __device__ __noinline__ void single_row(const PromptArgs& P, int b, int kh, long
     const unsigned short u = static_cast<unsigned short>(bits);
     return static_cast<float>(*reinterpret_cast<const T*>(&u));
   };
-  const uint2 q = lane * 4 < P.a.pool.Dh ? *reinterpret_cast<const uint2*>(static_cast<const T*>(P.a.q) + row * P.a.q_token + head * P.a.q_head + lane * 4) : make_uint2(0u, 0u);
+  const uint2 q = four_of<T>(P, P.a.q, row * P.a.q_token + head * P.a.q_head, lane);
   float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int p = lo; p <= pos; ++p) {
-    const uint2 k = four_of<T>(P, P.a.pool.k, b, kh, p, lane), v = four_of<T>(P, P.a.pool.v, b, kh, p, lane);
-    float s = 0.f;
-    for (int i = 0; i < 4; ++i) s = fmaf(number(q, i), number(k, i), s);
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= P.a.scale * 1.4426950408889634f;
-    const float m2 = fmaxf(m, s), ref = m2 == -INFINITY ? 0.f : m2, keep = exp2_fast(m - ref), w = exp2_fast(s - ref);
-    m = m2;
-    l = l * keep + w;
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * keep + w * number(v, i);
+  for (int p0 = lo; p0 <= pos; p0 += 32) {
+    const int n = min(32, pos - p0 + 1);
+    const long long at = lane < n ? place_of(P, b, kh, p0 + lane) : -1;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += kAtOnce) {
+      uint2 k[kAtOnce], v[kAtOnce];
+      float s[kAtOnce], m2 = m;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const long long there = __shfl_sync(0xffffffffu, at, i0 + i);
+        k[i] = four_of<T>(P, P.a.pool.k, there, lane);
+        v[i] = four_of<T>(P, P.a.pool.v, there, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        s[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) s[i] = fmaf(number(q, d), number(k[i], d), s[i]);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
+        s[i] = i0 + i < n ? s[i] * (P.a.scale * 1.4426950408889634f) : -INFINITY;
+        m2 = fmaxf(m2, s[i]);
+      }
+      const float ref = m2 == -INFINITY ? 0.f : m2, keep = exp2_fast(m - ref);
+      m = m2;
+      l *= keep;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[d] *= keep;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const float w = exp2_fast(s[i] - ref);
+        l += w;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[d] = fmaf(w, number(v[i], d), o[d]);
+      }
+    }
   }
   if (lane * 4 < P.a.pool.Dh)
     *reinterpret_cast<uint2*>(static_cast<T*>(P.a.out) + row * P.a.out_token + head * P.a.out_head + lane * 4) =
@@ -206,7 +245,10 @@ __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* v) {
 }
 
 // t5_wait for a converged warp whose lanes leave the loop together: 60 cycles where the barrier is ready; with a way out per lane 160.
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, uint32_t limit, unsigned int* err, volatile int* abort_flag) {
+// state: the block's word of kGivesUp and kMending for each of its warps that computes single rows again.  How long that takes depends on the
+// context, so while it lasts no wait's polls are counted; it waits for nothing itself, so it ends.
+constexpr int kGivesUp = 1, kMending = 2;
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, uint32_t limit, unsigned int* err, int* state) {
   const uint32_t addr = smem_addr(bar);
   for (uint32_t i = 0; i < limit; ++i) {
     uint32_t done;
@@ -218,10 +260,14 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, uint32
         : "r"(addr), "r"(parity)
         : "memory");
     if (__all_sync(0xffffffffu, done != 0)) return true;
-    if ((i & 63u) == 63u && __any_sync(0xffffffffu, *abort_flag != 0)) return false;
+    if ((i & 63u) == 63u) {
+      const int now = *static_cast<volatile int*>(state);
+      if (__any_sync(0xffffffffu, now & kGivesUp)) return false;
+      if (__any_sync(0xffffffffu, now != 0)) i = 0;
+    }
   }
   atomicOr(err, 1u);
-  *abort_flag = 1;
+  atomicOr(state, kGivesUp);
   return false;
 }
 
@@ -275,9 +321,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], mma_done[2], tail_full;
   __shared__ uint32_t tmem_slot[1];
-  __shared__ int abort_word, s_first[4];
+  __shared__ int state, s_first[4];
   __shared__ long long s_scan[kPromptThreads / 32], s_rest;
-  volatile int* abort_flag = &abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_addr(smem_raw), ring = base + 2 * Z::kTile;
   if (tid == 0) {
@@ -294,7 +339,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(smem_addr(mma_done + x), 1);
     }
     mbar_init(smem_addr(&tail_full), 1);
-    abort_word = 0;
+    state = 0;
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
@@ -427,7 +472,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         keys.step();
         values.step();
         if (!here) continue;   // the other tile's; this tile's issuing warp gives the stages back
-        if (!(ok = wait_warp(s_full + x, s_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+        if (!(ok = wait_warp(s_full + x, s_count++ & 1, P.wait_limit, P.a.err, &state))) break;
         if (leader) {
           mbar_arrive(empty + k_stage);
           if (j > r.first) mbar_arrive(empty + v_before);
@@ -498,7 +543,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (lane == 0) mbar_arrive(p_full + x);
       }
       if (!ok) break;   // of this warp; the others leave at their next wait
-      if (!r.none() && !(ok = wait_warp(o_full + x, o_count++ & 1, P.wait_limit, P.a.err, abort_flag))) break;
+      if (!r.none() && !(ok = wait_warp(o_full + x, o_count++ & 1, P.wait_limit, P.a.err, &state))) break;
       tc_fence_after();
       if (leader && !r.none()) mbar_arrive(empty + v_before);
       float check = 0.f;
@@ -562,12 +607,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(q_empty + x);
       }
-      for (; mend; mend &= mend - 1) {
-        const int src = __ffs(mend) - 1;
+      if (__builtin_expect(mend != 0, 0) && lane == 0) atomicAdd(&state, kMending);
+      for (uint32_t left = mend; left; left &= left - 1) {
+        const int src = __ffs(left) - 1;
         const int row_pos = __shfl_sync(0xffffffffu, pos, src), row_lo = __shfl_sync(0xffffffffu, lo, src);
         single_row<T>(P, p.b, p.h, p.s.row0 + p.t0 + x * P.tile_tokens + __shfl_sync(0xffffffffu, token, src),
                       p.h * P.group + __shfl_sync(0xffffffffu, head, src), row_lo, row_pos);
       }
+      if (__builtin_expect(mend != 0, 0) && lane == 0) atomicSub(&state, kMending);
       tc_fence_before();   // the next P is announced after these reads of O
     }
   } else {
@@ -603,7 +650,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               page = P.a.pool.n_pages;
             }
           }
-          if (!(ok = wait_warp(empty + s, ph ^ 1u, P.wait_limit, P.a.err, abort_flag))) break;
+          if (!(ok = wait_warp(empty + s, ph ^ 1u, P.wait_limit, P.a.err, &state))) break;
           const uint32_t stage = ring + s * Z::kTile;
           const bool cut = values && (end < kPosBlock || begin > 0);
           uint64_t* const bar = cut ? &tail_full : full + s;
@@ -620,7 +667,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
           }
           if (cut) {
-            ok = wait_warp(&tail_full, tails++ & 1, P.wait_limit, P.a.err, abort_flag);
+            ok = wait_warp(&tail_full, tails++ & 1, P.wait_limit, P.a.err, &state);
             uint8_t* dst = smem_raw + (stage - smem_addr(smem_raw));
             for (int n = lane; n < (kPosBlock - end + begin) * 8; n += 32) {   // rows end .. 127, then 0 .. begin - 1
               const int row = (end + (n >> 3)) & (kPosBlock - 1);
@@ -649,7 +696,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       Values values;
       bool ok = true, any = false;
       auto wait = [&](uint64_t* bar, int parity) -> bool {
-        if (ok) ok = wait_warp(bar, parity, P.wait_limit, P.a.err, abort_flag);
+        if (ok) ok = wait_warp(bar, parity, P.wait_limit, P.a.err, &state);
         tc_fence_after();
         return ok;
       };
@@ -737,7 +784,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   }
   // Every copy has been waited for by the multiplications, unless the block gave up: then those in flight land before it gives its
   // shared memory back (both parities: one of them has passed).
-  if (abort_word && warp == 0 && lane == 0) {
+  if ((state & kGivesUp) && warp == 0 && lane == 0) {
     for (int i = 0; i < kStages; ++i)
       for (int parity = 0; parity < 2; ++parity) mbar_wait(smem_addr(full + i), parity, P.a.err, 1u << 14);
     for (int x = 0; x < 2; ++x)

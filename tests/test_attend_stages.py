@@ -197,5 +197,5 @@ def test_a_block_that_gives_up_waits_for_every_copy():
     on = set(re.findall(r"mbar_expect\((\w+)", kernel))
     on |= set(re.findall(r"uint64_t\* const bar = cut \? &(\w+) : (\w+)", kernel)[0])
     assert on - {"bar"} == {"full", "q_full", "tail_full"}
-    gives_up = kernel[kernel.index("if (abort_word"):]
+    gives_up = kernel[kernel.index("// Every copy has been waited for"):]
     assert all(re.search(r"mbar_wait\(smem_addr\(&?%s\b" % name, gives_up) for name in on - {"bar"})

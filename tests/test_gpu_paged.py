@@ -271,6 +271,36 @@ def test_values_out_of_sight_do_not_show(lw, heads, length, new, window):
     assert torch.equal(~torch.isfinite(one[0]), shows[-1]) and torch.isfinite(one[1]).all()
 
 
+def test_rows_computed_again_do_not_run_out_the_waits(lw):
+    """Long contexts whose last value is infinite: the rows that do not see it are computed again, which takes far longer than the
+    waits of the block's other warps are given here; they must not give up meanwhile."""
+    import torch
+    from tests import paged_ref as ref
+    length, new, heads = 1500, 300, 32
+    pr = problem([length] * 5, [new] * 5, heads, heads, 64, 16, "fp16", seed=9)
+    for b in range(5):
+        v = ref.load(pr["v"], pr["table"], b, length)
+        v[length - 1, :, 5] = float("inf")
+        ref.store(pr["v"], pr["table"], b, 0, v)
+    cache = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+    args = [pr[n].cuda() for n in ("q", "table", "lens", "starts")]
+    lib = lw.lib()
+    try:
+        lib.lw_debug_set(b"wait_limit", 4000)
+        out = cache.attend_prompt(*args)
+        torch.cuda.synchronize()
+        assert lib.lw_kernel_error() == 0
+    finally:
+        lib.lw_debug_set(b"reset", 0)
+    out = out.cpu().double().view(5, new, heads, 64)
+    last = new - 256                            # rows of every sequence's second pair of tiles
+    for b in range(5):
+        k, v = (ref.load(pr[n], pr["table"], b, length)[:-1] for n in "kv")
+        want, bound, _ = ref.attend(pr["q"][(b + 1) * new - last:(b + 1) * new - 1], k, v, torch.arange(length - last, length - 1), 64 ** -0.5, 0)
+        assert ((out[b, -last:-1] - want).abs() <= bound).all()
+        assert torch.isinf(out[b, -1, :, 5]).all() and torch.isfinite(out[b, -1, :, 6:]).all()
+
+
 @pytest.mark.parametrize("window", [0, 40])
 @pytest.mark.parametrize("heads,length,new", [(2, 200, 200), (4, 300, 70), (2, 6000, 30), (1, 6000, 300)])
 def test_results_in_the_place_of_the_queries(lw, heads, length, new, window):
