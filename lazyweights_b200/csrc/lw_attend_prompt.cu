@@ -29,7 +29,8 @@
 //  * Values of positions that no row of the pair sees are zeroed in shared memory before they are multiplied (a weight of 0
 //    would not hide a NaN that an earlier owner of the page left).
 //  * Rounding: S, m, l, O in 32 bits; P in the cache's type, as the tensor core takes it (half a step of its 11 or 8 bits,
-//    independent from position to position); l adds the unrounded p.
+//    independent from position to position); l adds the unrounded p.  fp16 has no more than 2^-24 below 1, and a hundred thousand
+//    positions that small are a result's worth: p is taken times 2^kLift there (at most 2^(kSlack + kLift), in O and l alike).
 #include <cuda.h>
 
 #include <algorithm>
@@ -43,6 +44,7 @@ namespace lw {
 constexpr int kPromptThreads = 12 * 32;
 constexpr int kPromptRegsSoftmax = 216, kPromptRegsOther = 72;   // 8 and 4 warps: 12 x 168, the launch's
 constexpr float kSlack = 8.f;         // of a row's maximum, in powers of two, before its reference follows
+constexpr float kLift = 7.f;          // fp16: 2^15 is the largest power of two
 constexpr int kPromptLead = 2;       // 24 packed prompts of 20 to 2500 tokens: 234 us (0: 362, 1: 265, 3: 237)
 
 // The pair that block c continues: its first packed row, rows (tokens) and first query head, and the blocks that hold its first and
@@ -520,7 +522,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               }
             }
           }
-          const float ref = m == -INFINITY ? 0.f : m;
+          const float ref = m == -INFINITY ? 0.f : std::is_same<T, __half>::value ? m - kLift : m;
           const float2 c2 = make_float2(c, c), ref2 = make_float2(-ref, -ref);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll

@@ -20,7 +20,9 @@
 //    lengths, which it reads on the device.  What a worker begins or ends in the middle of goes to the workspace
 //    and is joined, in order, by k_token_join.
 //  * Positions outside the sequence or the window: scores replaced by -inf, values zeroed in shared memory (0 x NaN is NaN).
-//  * Rounding: scores, m, l, O in 32 bits, P in the cache's type for the tensor core (half a step of it, independent per position).
+//  * Rounding: scores, m, l, O in 32 bits, P in the cache's type for the tensor core (half a step of it, independent per position);
+//    in fp16 p is taken times 2^15, in O and l alike: its smallest number would otherwise be 2^-24 of the largest p, and a hundred
+//    thousand positions that small are a result's worth.
 #include <cuda.h>
 
 #include <algorithm>
@@ -390,7 +392,8 @@ __global__ void __launch_bounds__(kTokenThreads, kTokenBlocksPerSm)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[n][k][i] *= keep[i & 1];
         }
-        const float ref[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
+        constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
+        const float ref[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0] - kLift, m[n][1] == -INFINITY ? 0.f : m[n][1] - kLift};
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[n][i] = exp2_fast(x[n][i] - ref[i & 1]);
         l[n][0] += x[n][0] + x[n][2];

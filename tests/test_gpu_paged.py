@@ -169,6 +169,35 @@ def test_maxima_that_move(lw, order):
         check_attention(lw, pr, prompt=prompt)
 
 
+@pytest.mark.parametrize("prompt", [True, False])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("place", [0, 4000, 7999])
+def test_many_small_weights(lw, place, dtype, prompt):
+    """One position takes almost all of the weight and has values of 0; the 8000 others have e^-17 of its weight each, less than fp16
+    can tell from its neighbours 0 and 2^-24, and values of 1: together 0.0003, which is all there is of the result.  Enough
+    sequences (on the same pages) that most of them are not split."""
+    import math
+    import torch
+    from tests import paged_ref as ref
+    n, new, seqs = 8001, 3 if prompt else 1, 10 if prompt else 64
+    pr = problem([n], [new], 32, 32, 64, 16, dtype)
+    keys, values = torch.zeros(n, 32, 64), torch.ones(n, 32, 64)
+    keys[place, :, 0], values[place] = 17.0, 0.0
+    ref.store(pr["k"], pr["table"], 0, 0, keys), ref.store(pr["v"], pr["table"], 0, 0, values)
+    q = torch.zeros(seqs * new, 32, 64, dtype=dtypes()[dtype], device="cuda")
+    q[:, :, 0] = 1.0
+    cache = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+    table, lens = pr["table"].expand(seqs, -1).contiguous().cuda(), pr["lens"].expand(seqs).contiguous().cuda()
+    starts = torch.arange(0, seqs * new + 1, new, dtype=torch.int32, device="cuda")
+    out = (cache.attend_prompt(q, table, lens, starts, scale=1.0) if prompt else cache.attend(q, table, lens, scale=1.0)).cpu().double()
+    seen = [(pos + (pos < place), float(pos >= place)) for pos in range(n - new, n)]      # positions of value 1, and whether the heavy one is seen
+    want = torch.tensor([c * math.exp(-17.0) / (heavy + c * math.exp(-17.0)) for c, heavy in seen] * seqs, dtype=torch.float64)[:, None, None]
+    # weights: half a step of the type, or, lifted by 2^7, half of 2^-24 of 2^7 e^-17 = 2^-17.5 (2^-7.5 of it); exponentials 2^-13 of 32-bit scores of
+    # at most 17 log2(e) + 15 < 64 (2^-19); sums of n numbers in 32 bits, rounded to nearest or cut; the result's half step
+    rel = max(ref.EPS[dtypes()[dtype]], 2.0 ** -7.5) + 2 * (2.0 ** -13 + 2.0 ** -19) + 2 * n * 2.0 ** -23 + ref.EPS[dtypes()[dtype]]
+    assert ((out - want).abs() <= rel * want).all(), float(((out - want).abs() / want).max())
+
+
 def test_more_rows_than_positions(lw):
     """Rows before position 0 see nothing and give zeros."""
     import torch
