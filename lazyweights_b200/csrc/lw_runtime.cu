@@ -935,6 +935,7 @@ static double cfg_f(const Model* M, const char* k, double def) {
 
 template <class T>
 static int dalloc(Runtime* R, T** p, size_t count) {
+  if (debug_knobs().fail_alloc > 0 && --debug_knobs().fail_alloc == 0) return cuda_fail("cudaMalloc (runtime)", cudaErrorMemoryAllocation);
   const cudaError_t e = cudaMalloc(reinterpret_cast<void**>(p), std::max<size_t>(count, 1) * sizeof(T));
   if (e != cudaSuccess) return cuda_fail("cudaMalloc (runtime)", e);
   R->owned.push_back(*p);
@@ -1518,7 +1519,8 @@ int rt_pages(void* handle, int n_pages, int page_size) {
   }
   const size_t row = static_cast<size_t>(R->max_batch) * R->H * R->Dh;
   int rc;
-  if (!R->q16 && ((rc = dalloc(R, &R->q16, row)) || (rc = dalloc(R, &R->att16, row)))) return rc;
+  if (!R->q16 && (rc = dalloc(R, &R->q16, row))) return rc;   // each by itself: a call after a failed one makes what is missing
+  if (!R->att16 && (rc = dalloc(R, &R->att16, row))) return rc;
   if (!R->attn_space) {
     for (int prompt = 0; prompt < 2; ++prompt) R->attn_space_bytes = std::max(R->attn_space_bytes, lw_cache_workspace(R->caches[0], R->H, prompt));
     uint8_t* space = nullptr;

@@ -200,3 +200,27 @@ def test_numbers_that_do_not_fit_are_refused(tmp_path):
                 b.forward_seqs(*args)
         want = b.forward_seqs([ids.astype(np.int32)], [4], [[0]])
         assert np.array_equal(b.forward_seqs([ids], np.array([4]), np.array([[0]])), want)
+
+
+@pytest.mark.gpu
+def test_pages_after_a_failed_allocation(tmp_path):
+    """open_pages that ran out of memory at any of its buffers (the handle's test switch refuses it on the host) can be called again."""
+    helpers.build_library()
+    import lazyweights_b200 as lw
+    ids = [np.arange(5, dtype=np.int32), np.arange(2, dtype=np.int32)]
+    path, table = _model(tmp_path, 8, 2, 64)[0], [[1], [0]]
+    with lw.Bundle(path, max_ctx=64, max_batch=8) as b:
+        b.open_pages(3, 16)
+        want = b.forward_seqs(ids, [5, 2], table)
+    for n in (1, 2, 3):
+        with lw.Bundle(path, max_ctx=64, max_batch=8) as b:
+            try:
+                assert lw.lib().lw_debug_set(b"fail_alloc", n) == 0
+                with pytest.raises(lw.LwError):
+                    b.open_pages(3, 16)
+            finally:
+                lw.lib().lw_debug_set(b"reset", 0)
+            with pytest.raises(lw.LwError):
+                b.forward_seqs(ids, [5, 2], table)                  # no pages
+            b.open_pages(3, 16)
+            assert np.array_equal(b.forward_seqs(ids, [5, 2], table), want), n
