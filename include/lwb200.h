@@ -101,7 +101,9 @@ int rt_decode_greedy(void* handle, int first_token, int n, int* out);
  * ids[starts[b + 1] - 1] (starts[0] = 0; one at least per sequence, max_batch at most in all), the last of its lens[b] positions;
  * its pages are table[b * table_cols + 0 ..], which the caller gives out - two sequences may share the pages of a common
  * beginning.  logits (host, may be NULL): [n_seqs][vocab], of the last token of every sequence.  All arrays are host arrays, checked before
- * anything is launched.  The position of rt_forward and its own cache are not touched; rt_set_window applies.  0 or a negative status. */
+ * anything is launched.  The position of rt_forward and its own cache are not touched; rt_set_window applies.  Queries, attention's weights
+ * and its results are rounded to fp16 here (lw_cache_attend below; keys and values are in both), where rt_forward holds them in 32 bits: logits
+ * differ by those roundings, and a query beyond 65504 is infinite.  0 or a negative status. */
 int rt_pages(void* handle, int n_pages, int page_size);
 int rt_forward_seqs(void* handle, int n_seqs, const int* ids, const int* starts, const int* lens, const int* table, int table_cols,
                     float* logits);
@@ -304,7 +306,11 @@ long long lw_host_pairs(const uint8_t* codes, int N, int K, int fmt, const uint8
  * are read on the device, when the kernel runs: a captured call can be replayed with other lengths, pages and rows.
  * A page index outside the pool, a length beyond the table's columns or a position beyond the rotation tables is not
  * followed: nothing is written there, what is read there is undefined, and bit 1 of the device error word (lw_kernel_error) is
- * set.  All pointers but the handle are device pointers; calls launch on `stream` and do not synchronise. */
+ * set.  All pointers but the handle are device pointers; calls launch on `stream` and do not synchronise.  A call has at least one
+ * sequence and one row, and 2^30 rows at most.
+ * What is held in fewer than 32 bits: keys, values, queries and results in the cache's type (one rounding each, so beyond 65504 in fp16
+ * they are infinite), and attention's weights, which are rounded to that type before they meet the values (half a step of 11 or 8 bits each,
+ * independent of one another).  Scores, maxima and sums have 32 bits, as do the weights in the sum that divides. */
 enum { LW_TYPE_F16 = 0, LW_TYPE_BF16 = 1, LW_TYPE_F32 = 2 };
 
 /* A handle on two pools (nothing is allocated on the device).  n_kv_heads >= 1, page_size a multiple of 8 up to 65536, head_dim a

@@ -14,16 +14,16 @@
 // 1024 of exponentials (16 per cycle and SM).  So two tiles of 128 rows (a pair) share the staged keys and values of a thread block and
 // take turns: while one tile's softmax runs the tensor core works for the other.  What a block of positions takes now, 3350
 // cycles for both tiles, is the chain of one tile: 2000 cycles of softmax (scores in 450, exponentials 1400: the special-function
-// unit serves both tiles), then its multiplications and two hand-overs.  16384 tokens, 32 heads over 8: 2.0 to 2.2 ms with
-// the card's clock under its power limit, 1000 to 1100 TFLOP/s of what the mask leaves; 509 tokens behind 32000: 253 us, 1065.
+// unit serves both tiles), then its multiplications and two hand-overs.  Medians, with the clock that the card's power limit
+// leaves: 16384 tokens, 32 heads over 8: 2.26 ms at 1.63 GHz, 970 TFLOP/s of what the mask leaves; 509 tokens behind 32000: 305 us at 1.57, 880.
 //  * Warp 0 loads keys and warp 2 values (TMA; a page's rows of a kv head are a box), each into a ring of stages of its own: a wait's
 //    parity tells only neighbouring turns of a stage apart, so whoever loads one has to load every turn of it.  Warps 1 and 3 issue the
 //    multiplications of a tile each, and load its queries: issuing blocks while the tensor core is busy, and a commit costs it 78
 //    cycles, so one warp for both tiles with commits for the stages left it idle a third more.  Warps 4..7 and 8..11 are the softmax
 //    of the two tiles; they tell when a stage is read, from the completion of the scores behind it.
 //  * A thread holds a whole row of S, 128 registers: with two threads per row the exponentials took as long (the special-function unit) and
-//    the maximum had to be exchanged.  A third of the exponentials as polynomials on the other pipes changed nothing: the warps are
-//    bound by what they issue.  P handed over in halves made the exponentials slower than it made the product earlier.
+//    the maximum had to be exchanged.  A third of the exponentials as polynomials on the other pipes changed nothing: with a warp per tile
+//    and scheduler, each waiting for its own last instruction, the issue slots are 38 % busy and no pipe is full.  P handed over in halves made the exponentials slower than it made the product earlier.
 //  * The work is cut into equal shares whatever the lengths (lw_attend_plan.h), a pair's start and end counted as kPromptLead blocks
 //    of positions; a pair that is cut leaves unnormalised partial results, which k_attend_join adds up.  Lengths are read on the device.
 //  * Values of positions that no row of the pair sees are zeroed in shared memory before they are multiplied (a weight of 0
@@ -45,7 +45,7 @@ constexpr int kPromptThreads = 12 * 32;
 constexpr int kPromptRegsSoftmax = 216, kPromptRegsOther = 72;   // 8 and 4 warps: 12 x 168, the launch's
 constexpr float kSlack = 8.f;         // of a row's maximum, in powers of two, before its reference follows
 constexpr float kLift = 7.f;          // fp16: 2^15 is the largest power of two
-constexpr int kPromptLead = 2;       // 24 packed prompts of 20 to 2500 tokens: 234 us (0: 362, 1: 265, 3: 237)
+constexpr int kPromptLead = 2;       // 24 packed prompts of 20 to 2500 tokens: 243 us (0: 373, 1: 274, 3: 246); 16384 tokens: 2.27 ms (2.39, 2.35, 2.25)
 
 // The pair that block c continues: its first packed row, rows (tokens) and first query head, and the blocks that hold its first and
 // last unit (first == c: none).  A block leaves the pair that it continues as its piece 0, the one that it only begins as piece 1.
@@ -629,7 +629,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       uint32_t ph = 0;
       bool ok = true;
       constexpr int kHalves = DP / 64;
-      const int per_block = kPosBlock / P.box_rows;   // at most 16
       while (walk.left > 0 && ok) {
         const Piece p = next_piece(P, shape, walk);
         if (p.j0 == p.j1) continue;

@@ -21,7 +21,7 @@ namespace lw {
 // i < R, values past 2 R are copied; queries go to q_out, keys and values to their page.  fp32 arithmetic, one rounding.
 //
 // Bound: the row read once, written once (2 R = Dh = 128, 32 + 2 x 8 heads: 24 KB + 12 KB a row from fp32); at a row
-// or two, the chain of dependent loads starts -> length -> page.  Measured: 13555 such rows in 82 us, 6.16 TB/s, 94 % of a copy; one row 2.5 us.
+// or two, the chain of dependent loads starts -> length -> page.  Measured: 13555 such rows in 85 us, 5.96 TB/s, 91 % of a copy; one row 2.5 us.
 //  * A block per row, whose fixed thread handles unit u (8 values: four pairs, or eight copied ones) of every n-th head, so the
 //    tables are read once per thread, not once per head.  The row's values are requested before the block looks
 //    its sequence up: the two latencies overlap.

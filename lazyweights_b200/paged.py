@@ -9,7 +9,8 @@ with other contents):
   lens    [n]           length of every sequence, the positions of the call's rows included
   starts  [n + 1]       rows starts[b] .. starts[b + 1] - 1 are the last positions of sequence b; rows outside belong to none
 
-torch is only used for device memory and streams.  A page outside the pool, a length beyond the table or a position beyond
+Every call has at least one sequence and one row, and 2^30 rows at most.  Queries, keys, values, results and attention's weights are rounded to the cache's type, scores
+and sums held in 32 bits.  torch is only used for device memory and streams.  A page outside the pool, a length beyond the table or a position beyond
 the rotation tables is not followed and sets bit 1 of lw_kernel_error().
 """
 from . import _native as nat

@@ -275,7 +275,7 @@ class Bundle(_Handle):
     def forward_seqs(self, ids, lens, table):
         """rt_forward_seqs: one pass over the new tokens of several sequences.  ids: a list of their token arrays, lens: their lengths
         with the new tokens, table: [n, columns] their pages.  Returns the logits of every sequence's last token [n, vocab] (host
-        float32)."""
+        float32); queries and attention pass through fp16 where forward() holds them in 32 bits."""
         parts = [_int32(i, "ids").reshape(-1) for i in ids]
         starts = np.cumsum([0] + [p.size for p in parts]).astype(np.int32)
         flat = np.concatenate(parts) if parts else np.zeros(0, np.int32)
