@@ -14,6 +14,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// In fp16 weights are taken times 2^lift (most), so that small ones are not lost below its 2^-24; not where scores are so large that 32 bits
+// have no digits left for it and a weight could round beyond fp16.  `reference`: what scores are taken from, which is what O and l go by.
+constexpr float kLiftLimit = 4194304.f;   // 2^22: whole and quarter numbers are exact below
+template <typename T>
+__device__ __forceinline__ float lift(float reference, float most) {
+  return std::is_same<T, __half>::value && fabsf(reference) < kLiftLimit ? most : 0.f;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>

@@ -4,7 +4,7 @@
 //
 // One pass over the positions with a running reference m of the scores (in powers of two): p = 2^(c s - m), l = sum p,
 // O = sum p V; m is the row's maximum so far, moved only when the maximum has grown by more than kSlack, so that O and l are rescaled a
-// few times per row, not at every block (p stays below 2^kSlack, far inside fp16's range; O / l does not depend on m).
+// few times per row, not at every block (p stays below 2^(kSlack + kLift), inside fp16's range; O / l does not depend on m).
 //
 //  S = Q K^T    tcgen05.mma, both operands in shared memory       [128 rows x 128 positions], fp32 in tensor memory
 //  P            one thread per row reads S, writes P in the cache's type over S
@@ -30,7 +30,7 @@
 //    would not hide a NaN that an earlier owner of the page left).
 //  * Rounding: S, m, l, O in 32 bits; P in the cache's type, as the tensor core takes it (half a step of its 11 or 8 bits,
 //    independent from position to position); l adds the unrounded p.  fp16 has no more than 2^-24 below 1, and a hundred thousand
-//    positions that small are a result's worth: p is taken times 2^kLift there (at most 2^(kSlack + kLift), in O and l alike).
+//    positions that small are a result's worth: p is taken times 2^kLift there, m being that much less than the maximum it follows.
 #include <cuda.h>
 
 #include <algorithm>
@@ -44,7 +44,7 @@ namespace lw {
 constexpr int kPromptThreads = 12 * 32;
 constexpr int kPromptRegsSoftmax = 216, kPromptRegsOther = 72;   // 8 and 4 warps: 12 x 168, the launch's
 constexpr float kSlack = 8.f;         // of a row's maximum, in powers of two, before its reference follows
-constexpr float kLift = 7.f;          // fp16: 2^15 is the largest power of two
+constexpr float kLift = 7.f;          // fp16, whose largest power of two is 2^15
 constexpr int kPromptLead = 2;       // 24 packed prompts of 20 to 2500 tokens: 243 us (0: 373, 1: 274, 3: 246); 16384 tokens: 2.27 ms (2.39, 2.35, 2.25)
 
 // The pair that block c continues: its first packed row, rows (tokens) and first query head, and the blocks that hold its first and
@@ -505,9 +505,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
           for (int i = 0; i < 128; i += 2) mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
           const float mx = max3(max3(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * c;
-          const bool grow = mx > m + kSlack;
+          const bool grow = mx > m + kSlack + lift<T>(m, kLift);
           if (__any_sync(0xffffffffu, grow)) {
-            const float m2 = grow ? mx : m, keep = m == -INFINITY ? 0.f : exp2_fast(m - m2);   // nothing seen yet: O and l count for nothing
+            const float m2 = grow ? mx - lift<T>(mx, kLift) : m, keep = m == -INFINITY ? 0.f : exp2_fast(m - m2);   // nothing seen yet: O and l count for nothing
             m = m2;
             l *= keep;
             if (j > r.first) {   // PV of the block before is done: its completion came with these scores
@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               }
             }
           }
-          const float ref = m == -INFINITY ? 0.f : std::is_same<T, __half>::value ? m - kLift : m;
+          const float ref = m == -INFINITY ? 0.f : m;
           const float2 c2 = make_float2(c, c), ref2 = make_float2(-ref, -ref);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll

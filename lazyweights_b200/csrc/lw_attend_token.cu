@@ -21,8 +21,8 @@
 //    and is joined, in order, by k_token_join.
 //  * Positions outside the sequence or the window: scores replaced by -inf, values zeroed in shared memory (0 x NaN is NaN).
 //  * Rounding: scores, m, l, O in 32 bits, P in the cache's type for the tensor core (half a step of it, independent per position);
-//    in fp16 p is taken times 2^15, in O and l alike: its smallest number would otherwise be 2^-24 of the largest p, and a hundred
-//    thousand positions that small are a result's worth.
+//    in fp16 p is taken times 2^15, in O, l and the m of partial results alike: its smallest number would otherwise be 2^-24 of the
+//    largest p, and a hundred thousand positions that small are a result's worth.
 #include <cuda.h>
 
 #include <algorithm>
@@ -35,6 +35,7 @@ namespace lw {
 constexpr int kTokenWarps = 4, kTokenThreads = kTokenWarps * 32;
 constexpr int kUnit = 16;                 // positions of a unit
 constexpr int kTokenBlocksPerSm = 2;
+constexpr float kLift = 15.f;             // fp16: its largest power of two
 constexpr int kLead = 2;                  // see above: 200 sequences of 10 to 500 positions, 8 kv heads: 32.1 us (0: 41.7, 1: 34.5, 4: 32.5)
 
 // The piece that worker w continues: sequence, head slot, the workers that hold its first and last unit (first == w: none).
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(kTokenThreads, kTokenBlocksPerSm)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float m2 = fmaxf(m[n][e], mx[e]);
-            keep[e] = m[n][e] == -INFINITY ? 0.f : exp2_fast(m[n][e] - m2);
+            keep[e] = m[n][e] == -INFINITY ? 0.f : exp2_fast((m[n][e] - lift<T>(m[n][e], kLift)) - (m2 - lift<T>(m2, kLift)));
             m[n][e] = m2;
             l[n][e] *= keep[e];
           }
@@ -392,8 +393,7 @@ __global__ void __launch_bounds__(kTokenThreads, kTokenBlocksPerSm)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[n][k][i] *= keep[i & 1];
         }
-        constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
-        const float ref[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0] - kLift, m[n][1] == -INFINITY ? 0.f : m[n][1] - kLift};
+        const float ref[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0] - lift<T>(m[n][0], kLift), m[n][1] == -INFINITY ? 0.f : m[n][1] - lift<T>(m[n][1], kLift)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[n][i] = exp2_fast(x[n][i] - ref[i & 1]);
         l[n][0] += x[n][0] + x[n][2];
@@ -431,7 +431,9 @@ __global__ void __launch_bounds__(kTokenThreads, kTokenBlocksPerSm)
           store_heads<T>(out, P.a.out_head, heads - n * 8, P.a.pool.Dh, k, v, lane);
         }
       } else {
-        if (lane < 4) *reinterpret_cast<float4*>(part + (n * 8 + lane * 2) * 2) = make_float4(m[n][0], l[n][0], m[n][1], l[n][1]);
+        if (lane < 4)
+          *reinterpret_cast<float4*>(part + (n * 8 + lane * 2) * 2) =
+              make_float4(m[n][0] - lift<T>(m[n][0], kLift), l[n][0], m[n][1] - lift<T>(m[n][1], kLift), l[n][1]);
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
           *reinterpret_cast<float4*>(part + Z::kPartHead + ((n * kSteps + k) * 32 + lane) * 4) = make_float4(o[n][k][0], o[n][k][1], o[n][k][2], o[n][k][3]);

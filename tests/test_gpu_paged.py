@@ -198,6 +198,40 @@ def test_many_small_weights(lw, place, dtype, prompt):
     assert ((out - want).abs() <= rel * want).all(), float(((out - want).abs() / want).max())
 
 
+@pytest.mark.parametrize("prompt", [True, False])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("score", [2.0 ** 20, 2.9e6, 2.91e6, 2.0 ** 22, 2.0 ** 23 + 2.0 ** 15, 1.2e7, 2.0e7, 4.1e7, 8.0e7, -2.0e7])
+def test_scores_of_millions(lw, score, dtype, prompt):
+    """Three positions share the largest score, far from all others: the result is the mean of their values, however few digits 32 bits
+    leave a score of that size; also where the maximum moves through such sizes on the way, and where the work is split."""
+    import torch
+    from tests import paged_ref as ref
+    t = dtypes()[dtype]
+    lens = [300, 700, 6000]
+    pr = problem(lens, [40] * 3 if prompt else [1] * 3, 4, 2, 64, 16, dtype, seed=3)
+    places = [5, 133, 250]
+    pr["q"].zero_()
+    pr["q"][:, :, 0] = 4096.0
+    for b, n in enumerate(lens):
+        # before position 250 ever larger ones, all behind it far smaller; the three the largest
+        keys = torch.zeros(n, 2, 64)
+        other = score / 4096 * (torch.linspace(0.1, 0.8, n) if score > 0 else torch.linspace(1.8, 1.2, n))
+        keys[:, :, 0] = other[:, None]
+        keys[places, :, 0] = score / 4096
+        ref.store(pr["k"], pr["table"], b, 0, keys)
+    cache = lw.PagedCache(pr["k"].cuda(), pr["v"].cuda())
+    args = [pr[m].cuda() for m in ("q", "table", "lens")]
+    out = (cache.attend_prompt(*args, pr["starts"].cuda(), scale=1.0) if prompt else cache.attend(*args, scale=1.0)).cpu().double()
+    rows = 40 if prompt else 1
+    for b, n in enumerate(lens):
+        seen = min(n - rows + 1, n)                                             # every row sees the three
+        assert seen > max(places)
+        v = ref.load(pr["v"], pr["table"], b, n)[places].repeat_interleave(2, 1)   # [3, heads, dim]
+        want, size = v.mean(0), v.abs().mean(0)
+        # the three weights are equal, rounded alike (half a step) against an unrounded sum; the result's half step; 32-bit sums
+        assert ((out[b * rows:(b + 1) * rows] - want).abs() <= size * (2 * ref.EPS[t] + 2.0 ** -20)).all(), (b, n)
+
+
 def test_more_rows_than_positions(lw):
     """Rows before position 0 see nothing and give zeros."""
     import torch
